@@ -41,6 +41,12 @@ extern "C" {
 /* ---- element types ------------------------------------------------------------------- */
 #define VCSRMC_F32 0
 #define VCSRMC_F16 1
+#define VCSRMC_BF16 2 /* dense matrices of the microscaled operators                       */
+/* Microscaled (MX) matrices: elements of 8 or 4 bits and one power-of-two scale byte (E8M0:
+ * 2^(code - 127), 255 = NaN) for every 32 consecutive columns of a row; a row's last block may be
+ * shorter. Elements and scales are two arrays with row strides of their own, in bytes.          */
+#define VCSRMC_MXF8 3 /* E4M3 elements, one byte each                                       */
+#define VCSRMC_MXF4 4 /* E2M1 elements, two per byte, the even column in the low half       */
 
 /* ---- execution plans (vcsrmc_upload_ex / vcsrmc_spmm_ex) ------------------------------
  * SEGMENT: the reference's dataflow (src/vcsr_mc.cu:143-329): per work item, stage the B
@@ -250,6 +256,53 @@ int vcsrmc_spmm_ex(const vcsrmc_device_format* d, const void* B, int b_dtype, in
 int vcsrmc_spmm_timed(const vcsrmc_device_format* d, const void* B, int b_dtype, int64_t ldb,
                       int32_t O, int32_t tileK, float* C, int64_t ldc, int accumulate,
                       void* stream, float* ms);
+
+/* ---- microscaled (MX) dense operands (no reference counterpart) -------------------------
+ * A product gathers a row of B per entry of A, so the bytes of B bound it; an MX operand holds them
+ * in 8 or 4 bits. The pointer-only calls run on the calling thread's current device; all are
+ * asynchronous on `stream` and allocate nothing. Dense types are F32, F16 and BF16; pointers are
+ * aligned to their element type; row strides are in elements for dense matrices and in bytes for
+ * MX elements (ldq) and scales (lds). O is in [1, 2^30] (products: [1, 8388480]). Outputs must not
+ * overlap inputs unless a call says so; bytes between a row's end and its stride are left as they
+ * are.
+ *
+ * Q = MX(X): the scale of a block is the smallest power of two (at least 2^-127) under which its
+ * largest magnitude fits the element type (448 for E4M3, 6 for E2M1), so nothing is clipped; elements
+ * are rounded to nearest, ties to even. A block with an infinity or a NaN gets the NaN scale and zero
+ * elements; a block of zeros gets code 0. */
+int vcsrmc_mx_quantize(const void* X, int x_dtype, int64_t ldx, int64_t rows, int32_t O, int q_dtype,
+                       void* Q, int64_t ldq, uint8_t* S, int64_t lds, void* stream);
+/* Y = the values Q stands for (element * scale, rounded to Y's type). */
+int vcsrmc_mx_dequantize(const void* Q, int q_dtype, int64_t ldq, const uint8_t* S, int64_t lds,
+                         int64_t rows, int32_t O, void* Y, int y_dtype, int64_t ldy, void* stream);
+/* C[M x O] (+)= A * B with an MX operand B (N rows): both formats, ROWS layout, fp32 sums whose order
+ * is fixed (the same call gives the same bits). |a| * 2^(code - 127) of an entry and a block must be
+ * finite. The workspace (vcsrmc_spmm_mx_workspace bytes, 0 for a matrix without split rows; 16-byte
+ * aligned) is the caller's, so products of one handle may be in flight on several streams or in several
+ * graphs as long as each has its own; it need not be initialised. */
+int vcsrmc_spmm_mx_workspace(const vcsrmc_device_format* d, int32_t O, int64_t* bytes);
+int vcsrmc_spmm_mx(const vcsrmc_device_format* d, const void* Q, int q_dtype, int64_t ldq,
+                   const uint8_t* S, int64_t lds, int32_t O, float* C, int64_t ldc, int accumulate,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+/* Between two products: s = X + residual, rounded to the residual's type and stored in residual_out;
+ * inv_rms = 1 / sqrt(mean(s^2) + eps) of every row; Q = MX(s * inv_rms * weight). The residual (r_dtype)
+ * has X's type, or X is fp32, as a product's C. residual NULL: s = X; residual_out or inv_rms NULL: not
+ * stored. residual_out may be residual, or X where the types are the same, with the same stride. */
+int vcsrmc_add_rms_norm(const void* X, int x_dtype, int64_t ldx, const void* residual, int64_t ldr,
+                        void* residual_out, int64_t ldo, int r_dtype, const void* weight, int w_dtype,
+                        float eps, int64_t rows, int32_t O, int q_dtype, void* Q, int64_t ldq,
+                        uint8_t* S, int64_t lds, float* inv_rms, void* stream);
+/* Its gradients, with the elements' rounding taken as the identity: dY is the gradient of Q's values
+ * (fp32, or the residual's type), d_residual (may be NULL) that of residual_out, hidden the stored
+ * residual_out. dX (the residual's type) is the gradient of both X and residual, dweight (fp32, O values)
+ * that of the weight, summed in a fixed order. dX may be d_residual, or dY where the types are the same,
+ * with the same stride. The workspace is as for a product. */
+int vcsrmc_add_rms_norm_backward_workspace(int64_t rows, int32_t O, int64_t* bytes);
+int vcsrmc_add_rms_norm_backward(const void* dY, int dy_dtype, int64_t lddy, const void* d_residual,
+                                 int64_t lddr, const void* hidden, int64_t ldh, int r_dtype,
+                                 const void* weight, int w_dtype, const float* inv_rms, int64_t rows,
+                                 int32_t O, void* dX, int64_t lddx, float* dweight, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
 
 /* ---- synthetic inputs (no reference counterpart; the benchmark configurations) --------- */
 int vcsrmc_gen_csr(int kind, int32_t param, uint64_t seed, int nthreads, vcsrmc_csr** out);

@@ -1,0 +1,491 @@
+"""Microscaled (MX) operators on the GPU against the 64-bit definitions of mx_ref. Tolerances, u = 2^-24 (half a step of fp32, relative):
+  quantise and dequantise   exact (dequantise: one rounding to the output's type)
+  product                   fp32 sums of at most n terms and the factor of the FP16 format: (n + 4) u sum |a b|
+  norm                      y = s * inv * w from a 64-bit sum rounds four times: 4 u |y| before the element's own half step
+  backward                  half a step of dx's type and at most 8 roundings of its terms; dweight (rows + 4) u sum |dy s inv|"""
+import numpy as np
+import pytest
+import torch
+
+import vcsr_mc_b200 as vm
+from tests import mx_ref as ref
+from tests.helpers import random_csr
+
+pytestmark = pytest.mark.gpu
+KINDS = {"mxf8": vm.MXF8, "mxf4": vm.MXF4}
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = ref.U
+
+
+def np64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def codes_of(Q):
+    """(element codes, scale codes) of an MXDense."""
+    data, scale = Q.data.view(torch.uint8).cpu().numpy(), Q.scale.view(torch.uint8).cpu().numpy()
+    return (data[:, :Q.cols] if Q.kind == vm.MXF8 else ref.unpack(data, Q.cols)), scale[:, :-(-Q.cols // 32)]
+
+
+def to_mx(codes, scales, kind, pitch=None):
+    """An MXDense of given codes; pitch: bytes from one element row to the next."""
+    data = codes if kind == "mxf8" else ref.pack(codes)
+    wide = np.zeros((data.shape[0], pitch or data.shape[1]), np.uint8)
+    wide[:, :data.shape[1]] = data
+    d = torch.from_numpy(wide).cuda()[:, :data.shape[1]]
+    return vm.MXDense(d.view(torch.float8_e4m3fn) if kind == "mxf8" else d, torch.from_numpy(scales).cuda(), cols=codes.shape[1])
+
+
+def features(rows, O, seed, kind="mxf8"):
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((rows, O)) * np.exp2(rng.integers(-6, 7, (rows, 1)))
+    x[rng.random(rows) < 0.05] = 0
+    return ref.quantize(x.astype(np.float32), kind)
+
+
+# ---- quantise, dequantise --------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,O", [(1, 1), (3, 31), (5, 32), (7, 33), (4, 100), (129, 128), (2, 1009)])
+def test_quantize_exact(cuda, kind, dtype, rows, O):
+    rng = np.random.default_rng(rows * O)
+    spread = 120 if dtype != "f16" else 12
+    x = torch.from_numpy(rng.standard_normal((rows, O)) * np.exp2(rng.integers(-spread, spread, (rows, 1)))).to(TYPES[dtype]).cuda()
+    x[0, 0] = 0
+    codes, scales = ref.quantize(np64(x), kind)
+    Q = vm.mx_quantize(x, KINDS[kind])
+    got, got_s = codes_of(Q)
+    assert np.array_equal(got_s, scales) and np.array_equal(got, codes)
+    for t in TYPES.values():
+        want = torch.from_numpy(ref.values(codes, scales, kind).astype(np.float32)).to(t)
+        assert torch.equal(vm.mx_dequantize(Q, dtype=t).cpu(), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_quantize_borders(cuda, kind):
+    """Ties, the largest value of the type, one step beyond it, the ends of fp32, zeros, infinities and NaN."""
+    grid = ref._grid(kind)
+    mid = (grid[1:] + grid[:-1]) / 2
+    top = ref.LARGEST[kind]
+    rows = [np.append(mid[-31:], top), np.append(-mid[:31], top), np.append(np.nextafter(np.float32(mid[-31:]), np.float32(9e9)), top)]
+    rows += [np.full(32, v) for v in (0.0, -0.0, top, np.nextafter(np.float32(top), np.float32(1e9)), 1e-45, 2.0 ** -126, 2.0 ** -127, 3e38,
+                                      3.4028234663852886e38)]
+    rows += [np.append(np.ones(31), v) for v in (np.inf, -np.inf, np.nan)]
+    width = max(len(r) for r in rows)
+    x = np.stack([np.pad(r, (0, width - len(r))) for r in rows]).astype(np.float32)
+    codes, scales = ref.quantize(x, kind)
+    got, got_s = codes_of(vm.mx_quantize(torch.from_numpy(x).cuda(), KINDS[kind]))
+    assert np.array_equal(got_s, scales) and np.array_equal(got, codes)
+    assert (scales == 255).sum() == 3
+    back = vm.mx_dequantize(vm.mx_quantize(torch.from_numpy(x).cuda(), KINDS[kind])).cpu().numpy()
+    assert np.isnan(back[-3:]).all() and not np.isnan(back[:-3]).any()
+
+
+def test_dequantize_every_code(cuda):
+    all8, all4 = np.arange(256, dtype=np.uint8).reshape(8, 32), np.arange(16, dtype=np.uint8).reshape(1, 16)
+    for scale in (0, 1, 64, 127, 200, 254, 255):
+        for kind, codes in (("mxf8", all8), ("mxf4", all4)):
+            s = np.full((codes.shape[0], 1), scale, np.uint8)
+            got = vm.mx_dequantize(to_mx(codes, s, kind)).cpu().numpy()
+            with np.errstate(over="ignore"):
+                assert np.array_equal(got, ref.values(codes, s, kind).astype(np.float32), equal_nan=True)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shift,pitch", [(0, 144), (8, 144), (1, 133), (3, 131)])
+def test_quantize_strides(cuda, kind, shift, pitch):
+    """Rows and columns inside larger buffers, whatever their alignment; what lies around them stays."""
+    O = 97
+    x = torch.randn(6, pitch, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).half()
+    view = x[1:5, shift:shift + O]
+    nb = O if kind == "mxf8" else (O + 1) // 2
+    data = torch.full((6, pitch), 77, dtype=torch.uint8, device="cuda")
+    scale = torch.full((6, 9), 66, dtype=torch.uint8, device="cuda")
+    d = data[1:5, shift:shift + nb]
+    out = vm.MXDense(d.view(torch.float8_e4m3fn) if kind == "mxf8" else d, scale[1:5, 2:6], cols=O)
+    vm.mx_quantize(view, KINDS[kind], out=out)
+    codes, scales = ref.quantize(np64(view), kind)
+    got, got_s = codes_of(out)
+    assert np.array_equal(got, codes) and np.array_equal(got_s, scales)
+    data[1:5, shift:shift + nb] = 77
+    scale[1:5, 2:6] = 66
+    assert bool((data == 77).all()) and bool((scale == 66).all())
+    y = torch.full((6, pitch), 5.0, device="cuda", dtype=torch.bfloat16)
+    vm.mx_quantize(view, KINDS[kind], out=out)
+    vm.mx_dequantize(out, out=y[1:5, shift:shift + O])
+    want = torch.from_numpy(ref.values(codes, scales, kind)).float().bfloat16()
+    assert torch.equal(y[1:5, shift:shift + O].cpu(), want)
+    y[1:5, shift:shift + O] = 5
+    assert bool((y == 5).all())
+
+
+def test_no_rows(cuda):
+    for kind in KINDS.values():
+        Q = vm.mx_quantize(torch.zeros(0, 40, device="cuda"), kind)
+        assert Q.shape == (0, 40) and vm.mx_dequantize(Q).shape == (0, 40)
+        Q, h, inv = vm.add_rms_norm(torch.zeros(0, 40, device="cuda"), torch.ones(40, device="cuda"), kind=kind)
+        assert Q.shape == (0, 40) and inv.shape == (0,)
+    dx, dw = vm.add_rms_norm_backward(torch.zeros(0, 40, device="cuda"), torch.ones(40, device="cuda"), torch.zeros(0, 40, device="cuda"),
+                                      torch.zeros(0, device="cuda"))
+    assert dx.shape == (0, 40) and bool((dw == 0).all())
+
+
+# ---- product ---------------------------------------------------------------------------------------
+def sparse(M, N, density, seed, long_row=None, scale=1.0):
+    """CSR with fp16 values; every third row empty; `long_row`: that row holds every column."""
+    rp, col, val = random_csr(M, N, density, seed, empty_rows=True, scale=scale)
+    if long_row is not None:
+        rng = np.random.default_rng(seed + 1)
+        col = np.concatenate([col[:rp[long_row]], np.arange(N, dtype=np.int32), col[rp[long_row + 1]:]])
+        val = np.concatenate([val[:rp[long_row]], (rng.uniform(-1, 1, N) * scale).astype(np.float32), val[rp[long_row + 1]:]])
+        rp = rp.copy()
+        rp[long_row + 1:] += N - (rp[long_row + 1] - rp[long_row])
+    return rp, col.astype(np.int32), val.astype(np.float16).astype(np.float32)
+
+
+def handle(M, N, rp, col, val, fp32, built="upload", **kw):
+    if built == "upload":
+        V = vm.csr_to_vcsr_mc(vm.CSR.from_arrays(M, N, rp, col, val), fp32=fp32, segw=32)
+        return vm.upload_vcsr_mc_device(V, plans=[vm.PLAN_ROWS], **kw)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return vm.build_vcsr_mc_device(t(rp.astype(np.int32)), t(col), t(val), M, N, fp32=fp32, segw=32, plans=[vm.PLAN_ROWS], **kw)
+
+
+def check_product(dV, csr, codes, scales, kind, Q=None, start=None):
+    rp, col, val = csr
+    O = codes.shape[1]
+    B = ref.values(codes, scales, kind)
+    want, size, n = ref.product(rp, col, val, B)
+    C = torch.full((len(rp) - 1, O), 9.0, device="cuda") if start is None else start.clone()
+    vm.spmm(dV, to_mx(codes, scales, kind) if Q is None else Q, C, accumulate=start is not None)
+    if start is not None:
+        want, size = want + np64(start), size + np.abs(np64(start))
+    bound = (n + 4) * U * size
+    assert np.all(np.abs(np64(C) - want) <= bound), float(np.max(np.abs(np64(C) - want) - bound))
+    return C
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("fp32", [False, True])
+@pytest.mark.parametrize("O", [1, 2, 15, 16, 31, 32, 33, 64, 100, 127, 128, 129, 200, 256])
+def test_product_widths(cuda, kind, fp32, O):
+    M, N = 90, 70
+    csr = sparse(M, N, 0.2, O, long_row=4)
+    dV = handle(M, N, *csr, fp32, rows_unit_nnz=16)
+    codes, scales = features(N, O, O, kind)
+    C = check_product(dV, csr, codes, scales, kind)
+    start = torch.randn(M, O, device="cuda", generator=torch.Generator("cuda").manual_seed(O))
+    check_product(dV, csr, codes, scales, kind, start=start)
+    again = torch.empty_like(C)
+    vm.spmm(dV, to_mx(codes, scales, kind), again)
+    assert torch.equal(again, C), "the same call gives other bits"
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("M,N,density,unit,built", [(1, 1, 1.0, 0, "upload"), (1, 5000, 1.0, 0, "build"), (1, 5000, 1.0, 1024, "upload"),
+                                                    (2000, 1, 0.5, 0, "build"), (700, 900, 0.02, 0, "upload"), (700, 900, 0.02, 64, "build"),
+                                                    (50, 40, 0.0, 0, "upload"), (33, 3000, 0.3, 32, "build")])
+def test_product_shapes(cuda, kind, M, N, density, unit, built):
+    csr = sparse(M, N, density, M + N)
+    dV = handle(M, N, *csr, False, built, rows_unit_nnz=unit)
+    codes, scales = features(N, 72, M, kind)
+    check_product(dV, csr, codes, scales, kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("O,pitch,shift", [(128, 256, 0), (128, 160, 16), (128, 136, 8), (128, 132, 4), (128, 131, 0), (96, 129, 1), (64, 99, 2), (100, 112, 0),
+                                           (45, 61, 3)])
+def test_product_strides(cuda, kind, O, pitch, shift):
+    """B in a larger buffer at any alignment, its scales too; C in a larger buffer whose other columns and rows stay."""
+    M, N = 60, 50
+    csr = sparse(M, N, 0.3, O, long_row=0)
+    dV = handle(M, N, *csr, False, rows_unit_nnz=16)
+    codes, scales = features(N, O, pitch, kind)
+    data = codes if kind == "mxf8" else ref.pack(codes)
+    buf = torch.full((N + 2, pitch + 32), 0xFF, dtype=torch.uint8, device="cuda")
+    sbuf = torch.full((N + 2, 13), 0xFF, dtype=torch.uint8, device="cuda")
+    # a row stride of `pitch` bytes, starting `shift` bytes into the buffer
+    d = torch.as_strided(buf.view(-1), data.shape, (pitch, 1), pitch + shift)
+    s = sbuf[1:N + 1, 3:3 + scales.shape[1]]
+    d.copy_(torch.from_numpy(data))
+    s.copy_(torch.from_numpy(scales))
+    Q = vm.MXDense(d.view(torch.float8_e4m3fn) if kind == "mxf8" else d, s, cols=O)
+    want, size, n = ref.product(*csr, ref.values(codes, scales, kind))
+    for off, ldc in ((0, O), (1, O + 3), (4, O + 8), (8, O + 24)):
+        big = torch.full((M + 2, ldc + off), 3.5, device="cuda")
+        C = big[1:M + 1, off:off + O]
+        vm.spmm(dV, Q, C)
+        assert np.all(np.abs(np64(C) - want) <= (n + 4) * U * size)
+        C.fill_(3.5)
+        assert bool((big == 3.5).all())
+    # the first columns of a wider operand
+    C = torch.empty(M, O // 2, device="cuda")
+    vm.spmm(dV, Q, C, O=O // 2)
+    assert np.all(np.abs(np64(C) - want[:, :O // 2]) <= (n + 4) * U * size[:, :O // 2])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_product_special_values(cuda, kind):
+    """NaN scales reach exactly the rows and blocks that use them; unused and padded places reach nothing."""
+    M, N, O = 40, 64, 96
+    rp, col, val = sparse(M, N, 0.2, 3, long_row=5)  # 64 entries of row 5 in chunks of 16
+    keep = np.ones(len(col), bool)
+    keep[(col == 0) | (col == 7)] = False  # rows 0 and 7 of B are used by nobody
+    keep[rp[5] + 10:rp[5] + 13] = False    # row 5's last chunk is not whole
+    lens = np.array([keep[rp[r]:rp[r + 1]].sum() for r in range(M)])
+    col, val = col[keep], val[keep]
+    rp = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    dV = handle(M, N, rp, col, val, False, rows_unit_nnz=16)
+    codes, scales = features(N, O, 4, kind)
+    scales[0], scales[7] = 255, 255
+    if kind == "mxf8":
+        codes[0] = 0x7F
+    C = check_product(dV, (rp, col, val), codes, scales, kind)
+    assert bool(torch.isfinite(C).all())
+    scales[9, 1] = 255
+    C2 = torch.empty_like(C)
+    vm.spmm(dV, to_mx(codes, scales, kind), C2)
+    uses = np.array([9 in col[rp[r]:rp[r + 1]] for r in range(M)])
+    nan = torch.isnan(C2).cpu().numpy()
+    assert nan[uses][:, 32:64].all() and not nan[~uses].any() and not nan[:, :32].any() and not nan[:, 64:].any()
+
+
+def test_product_scaled_format_hot_columns_and_extremes(cuda):
+    M, N, O = 80, 60, 64
+    for scale in (1e6, 1e-7):
+        csr = sparse(M, N, 0.3, 5)
+        csr = (csr[0], csr[1], (csr[2] * np.float32(scale)).astype(np.float32))
+        V = vm.csr_to_vcsr_mc(vm.CSR.from_arrays(M, N, *csr), fp32=False, segw=32)
+        assert V.scale != 1.0
+        dV = vm.upload_vcsr_mc_device(V, plans=[vm.PLAN_ROWS])
+        held = ((csr[2] / np.float32(V.scale)).astype(np.float16).astype(np.float64) * np.float64(np.float32(V.scale)))
+        check_product(dV, (csr[0], csr[1], held), *features(N, O, 6, "mxf4"), "mxf4")
+    csr = sparse(M, N, 0.3, 5, long_row=2)
+    dV = handle(M, N, *csr, True, hot_rows=20)
+    assert dV.info()["n_hot"] > 0
+    check_product(dV, csr, *features(N, O, 6, "mxf4"), "mxf4")
+    # scales at both ends of their range, in different rows and blocks
+    codes, scales = features(N, O, 7, "mxf8")
+    scales[::2, 0], scales[1::2, 0], scales[:, 1] = 100, 4, 230
+    check_product(dV, csr, codes, scales, "mxf8")
+
+
+def test_product_refusals(cuda):
+    M, N = 20, 30
+    csr = sparse(M, N, 0.3, 5, long_row=1)
+    dV = handle(M, N, *csr, False, rows_unit_nnz=16)
+    codes, scales = features(N, 64, 1, "mxf8")
+    Q, C = to_mx(codes, scales, "mxf8"), torch.empty(M, 64, device="cuda")
+    short = to_mx(codes[:-1], scales[:-1], "mxf8")
+    for call in (lambda: vm.spmm(dV, short, C), lambda: vm.spmm(dV, Q, C[:-1]), lambda: vm.spmm(dV, Q, C, O=65),
+                 lambda: vm.spmm(dV, Q, C.half()), lambda: vm.spmm(dV, Q, C, plan=vm.PLAN_BAND), lambda: vm.spmm(dV, Q, C, tileK=77),
+                 lambda: vm.spmm(dV, Q, C.cpu()), lambda: vm.spmm(dV, Q, C, O=0)):
+        with pytest.raises(vm.VcsrmcError):
+            call()
+    from vcsr_mc_b200 import _lib
+    with pytest.raises(vm.VcsrmcError):  # no workspace for the split row
+        _lib.call("vcsrmc_spmm_mx", dV.handle, *Q._args(), 64, C.data_ptr(), 64, 0, None, 0, None)
+    only_segment = vm.upload_vcsr_mc_device(vm.csr_to_vcsr_mc(vm.CSR.from_arrays(M, N, *csr), segw=32), plans=[vm.PLAN_SEGMENT])
+    with pytest.raises(vm.VcsrmcError):
+        vm.spmm(only_segment, Q, C)
+    check_product(dV, csr, codes, scales, "mxf8")
+
+
+# ---- norm ------------------------------------------------------------------------------------------
+def check_norm(Q, inv, s, w, eps, kind):
+    y, want_inv = ref.norm(np64(s), np64(w), eps)
+    assert np.all(np.abs(np64(inv) - want_inv) <= 2 * U * want_inv)
+    codes, scales = codes_of(Q)
+    lo, hi = ref.scale_codes(y * (1 - 4 * U), kind), ref.scale_codes(y * (1 + 4 * U), kind)
+    assert np.all((scales >= lo) & (scales <= hi))
+    two = np.exp2(np.repeat(scales, 32, 1)[:, :y.shape[1]].astype(float) - 127)
+    got = ref.element_values(codes, kind)
+    grid = ref._grid(kind)
+    at = np.searchsorted(grid, np.abs(got))
+    up = np.append(grid, 2 * grid[-1] - grid[-2])[at + 1] - np.abs(got)
+    down = np.abs(got) - np.where(at > 0, grid[at - 1], -grid[1])
+    off = np.abs(y) / two - np.abs(got)
+    slack = 4 * U * np.abs(y) / two
+    assert np.all(off <= up / 2 + slack) and np.all(-off <= down / 2 + slack)
+    assert np.all((np.sign(got) == np.sign(y)) | (got == 0))
+
+
+COMBOS = [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")]
+WIDTHS = [1, 7, 32, 33, 64, 100, 128, 250, 256, 500, 1000, 1024, 1025, 2048, 4096, 5000, 16384, 32768, 32769, 40000]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("x,r", COMBOS)
+@pytest.mark.parametrize("O", WIDTHS)
+def test_norm(cuda, kind, x, r, O):
+    rows = 9 if O < 2000 else 3
+    g = torch.Generator("cuda").manual_seed(O)
+    X = torch.randn(rows, O, device="cuda", generator=g).to(TYPES[x])
+    R = (torch.randn(rows, O, device="cuda", generator=g) * 3).to(TYPES[r])
+    w = (1 + 0.2 * torch.randn(O, device="cuda", generator=g)).to(TYPES[r])
+    X[0], R[0] = 0, 0  # a row of zeros
+    Q, h, inv = vm.add_rms_norm(X, w, residual=R, eps=1e-5, kind=KINDS[kind])
+    s = (X.float() + R.float()).to(TYPES[r])
+    assert torch.equal(h, s)
+    check_norm(Q, inv, s, w, 1e-5, kind)
+    # in place on the residual, and a weight of another type
+    keep = R.clone()
+    Q2, h2, inv2 = vm.add_rms_norm(X, w.float(), residual=keep, eps=1e-5, kind=KINDS[kind], residual_out=keep)
+    assert h2.data_ptr() == keep.data_ptr() and torch.equal(keep, s) and torch.equal(inv2, inv)
+    assert torch.equal(Q2.data.view(torch.uint8), Q.data.view(torch.uint8)) and torch.equal(Q2.scale.view(torch.uint8), Q.scale.view(torch.uint8))
+    # without a residual
+    Q3, h3, inv3 = vm.add_rms_norm(X, w, eps=1e-5, kind=KINDS[kind])
+    assert h3 is X
+    check_norm(Q3, inv3, X, w, 1e-5, kind)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 63, 64, 65, 1000])
+def test_norm_rows_and_strides(cuda, rows):
+    O, ld = 72, 91
+    g = torch.Generator("cuda").manual_seed(rows)
+    X, R = torch.randn(rows, ld, device="cuda", generator=g)[:, 3:3 + O], torch.randn(rows, ld, device="cuda", generator=g).half()[:, 5:5 + O]
+    w = torch.randn(O, device="cuda", generator=g).half()
+    big = torch.full((rows + 2, ld), 2.0, device="cuda", dtype=torch.float16)
+    Q, h, inv = vm.add_rms_norm(X, w, residual=R, residual_out=big[1:rows + 1, 7:7 + O])
+    s = (X + R.float()).half()
+    assert torch.equal(h, s)
+    check_norm(Q, inv, s, w, 1e-6, "mxf8")
+    h.fill_(2.0)
+    assert bool((big == 2).all())
+
+
+def test_norm_extremes(cuda):
+    """Sums of squares that leave fp32's range, infinities and NaN stay in their rows."""
+    X = torch.ones(6, 64, device="cuda")
+    X[1] *= 1e25
+    X[2] *= 1e-25
+    X[3, 5] = float("inf")
+    X[4, 40] = float("nan")
+    w = torch.ones(64, device="cuda")
+    Q, _, inv = vm.add_rms_norm(X, w, eps=0.0)
+    keep = [0, 1, 2, 5]
+    check_norm(vm.MXDense(Q.data[keep].view(torch.uint8).view(torch.float8_e4m3fn), Q.scale.view(torch.uint8)[keep].contiguous()), inv[keep],
+               X[keep], w, 0.0, "mxf8")
+    y = vm.mx_dequantize(Q)
+    assert bool(torch.isnan(y[3, :32]).all()) and bool((y[3, 32:] == 0).all()) and bool(torch.isnan(y[4]).all())
+
+
+@pytest.mark.parametrize("x,r", COMBOS)
+@pytest.mark.parametrize("rows,O", [(1, 1), (5, 32), (70, 33), (300, 128), (2500, 100), (40, 1000), (17, 1025), (700, 2048), (6, 8192), (5, 16385), (3, 40000)])
+def test_norm_backward(cuda, x, r, rows, O):
+    g = torch.Generator("cuda").manual_seed(rows + O)
+    dY = torch.randn(rows, O, device="cuda", generator=g).to(TYPES[x])
+    dR, h = (torch.randn(rows, O, device="cuda", generator=g).to(TYPES[r]) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(O, device="cuda", generator=g)).to(TYPES[r])
+    h[0] = 0
+    inv = (1 / torch.sqrt(h.double().square().mean(1) + 1e-5)).float()
+    for d_residual in (dR, None):
+        dx, dw, size, dw_size = ref.norm_backward(np64(dY), np64(w), np64(h), np64(inv), None if d_residual is None else np64(d_residual))
+        got, got_w = vm.add_rms_norm_backward(dY, w, h, inv, d_residual=d_residual)
+        half = torch.finfo(TYPES[r]).eps / 2
+        tiny = float(torch.finfo(TYPES[r]).smallest_normal) * float(torch.finfo(TYPES[r]).eps)  # a step of the type's subnormals
+        assert got.dtype == TYPES[r] and got_w.dtype == torch.float32
+        assert np.all(np.abs(np64(got) - dx) <= half * np.abs(dx) + 8 * U * size * (1 + half) + tiny)
+        assert np.all(np.abs(np64(got_w) - dw) <= (rows + 4) * U * dw_size)
+        again, again_w = vm.add_rms_norm_backward(dY, w, h, inv, d_residual=d_residual)
+        assert torch.equal(again, got) and torch.equal(again_w, got_w)
+    place = dR.clone()
+    out, _ = vm.add_rms_norm_backward(dY, w, h, inv, d_residual=place, out=place)
+    assert out.data_ptr() == place.data_ptr()
+    want, _ = vm.add_rms_norm_backward(dY, w, h, inv, d_residual=dR)
+    assert torch.equal(place, want)
+
+
+def test_norm_backward_against_differences(cuda):
+    """The chain x -> norm -> values, through the library's own forward statistics, against differences of the 64-bit forward."""
+    g = torch.Generator("cuda").manual_seed(3)
+    X, R = (torch.randn(2, 40, device="cuda", generator=g) for _ in range(2))
+    w, G, D = torch.randn(40, device="cuda", generator=g), torch.randn(2, 40, device="cuda", generator=g), torch.randn(2, 40, device="cuda", generator=g)
+    _, h, inv = vm.add_rms_norm(X, w, residual=R, eps=1e-3)
+    dx, dw = vm.add_rms_norm_backward(G, w, h, inv, d_residual=D)
+    x, r, wd, gd, dd = (np64(t) for t in (X, R, w, G, D))
+
+    def loss(x, w):
+        s = x + r
+        return (ref.norm(s, w, 1e-3)[0] * gd).sum() + (s * dd).sum()
+
+    step = 1e-4  # differences: O(step^2) ~ 1e-7 of terms of order 10; fp32 results: 8 u of terms of order 10
+    for i in range(2):
+        for j in range(0, 40, 7):
+            d = np.zeros((2, 40))
+            d[i, j] = step
+            assert abs((loss(x + d, wd) - loss(x - d, wd)) / (2 * step) - float(dx[i, j])) < 1e-4
+    for j in range(40):
+        d = np.zeros(40)
+        d[j] = step
+        assert abs((loss(x, wd + d) - loss(x, wd - d)) / (2 * step) - float(dw[j])) < 1e-4
+
+
+# ---- together ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS)
+def test_layers_run_captured_and_on_streams(cuda, kind):
+    """Products and norms in turn over one matrix, as feature propagation uses them: eagerly, captured in two graphs that replay in turn
+    and on two streams at once, always to the same bits; and the way back through the transposed matrix."""
+    M, O = 400, 96
+    rp, col, val = sparse(M, M, 0.03, 8, long_row=3)
+    dV = handle(M, M, rp, col, val, False, rows_unit_nnz=32)
+    g = torch.Generator("cuda").manual_seed(4)
+    X0, w = torch.randn(M, O, device="cuda", generator=g).half(), torch.ones(O, device="cuda", dtype=torch.float16)
+
+    def layers(X):
+        C = torch.empty(M, O, device="cuda")
+        h, Q = X, vm.mx_quantize(X, KINDS[kind])
+        for _ in range(3):
+            vm.spmm(dV, Q, C)
+            Q, h, inv = vm.add_rms_norm(C, w, residual=h, kind=KINDS[kind])
+        return C, h, inv
+
+    eager = layers(X0)
+    # layer by layer against the definitions, from the library's own inputs of each step
+    Q = vm.mx_quantize(X0, KINDS[kind])
+    C = check_product(dV, (rp, col, val), *codes_of(Q), kind)
+    Q, h, inv = vm.add_rms_norm(C, w, residual=X0, kind=KINDS[kind])
+    check_norm(Q, inv, (C + X0.float()).half(), w, 1e-6, kind)
+    graphs = []
+    torch.cuda.synchronize()
+    for _ in range(2):
+        X = X0.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            layers(X)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layers(X)
+        graphs.append((graph, X, out))
+    graphs[1][1].copy_(X0 * 2)
+    two = layers(X0 * 2)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(s1):
+            graphs[0][0].replay()
+        with torch.cuda.stream(s2):
+            graphs[1][0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(graphs[0][2], eager)) and all(torch.equal(a, b) for a, b in zip(graphs[1][2], two))
+    # an explicit stream that is not the current one
+    s1.wait_stream(torch.cuda.current_stream())
+    Q = vm.mx_quantize(X0, KINDS[kind], stream=s1)
+    C = torch.empty(M, O, device="cuda")
+    s1.wait_stream(torch.cuda.current_stream())
+    vm.spmm(dV, Q, C, stream=s1.cuda_stream)
+    s1.synchronize()
+    first = torch.empty_like(C)
+    vm.spmm(dV, vm.mx_quantize(X0, KINDS[kind]), first)
+    assert torch.equal(C, first)
+    # back: dB = A^T dC, with dC microscaled
+    order = np.argsort(col, kind="stable")
+    rows = np.repeat(np.arange(M), np.diff(rp))[order]
+    rpt = np.concatenate([[0], np.cumsum(np.bincount(col, minlength=M))]).astype(np.int32)
+    dT = handle(M, M, rpt, rows.astype(np.int32), val[order], False)
+    dC = vm.mx_quantize(torch.randn(M, O, device="cuda", generator=g), KINDS[kind])
+    dB = check_product(dT, (rpt, rows, val[order]), *codes_of(dC), kind)
+    dx, dw = vm.add_rms_norm_backward(dB, w, eager[1], eager[2])
+    assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dw).all())

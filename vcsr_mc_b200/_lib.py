@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libvcsrmc.so")
 
 # status codes (vcsrmc.h)
 OK, INVALID_ARG, CUDA_ERR, OOM, TIMEOUT, IO_ERR, FORMAT_ERR, INTERNAL = range(8)
-F32, F16 = 0, 1
+F32, F16, BF16, MXF8, MXF4 = range(5)
 GEN_UNIFORM_POISSON, GEN_ZIPF, GEN_STENCIL27, GEN_RMAT, GEN_STENCIL27_LINKS = 1, 2, 3, 4, 5
 PLAN_AUTO, PLAN_SEGMENT, PLAN_ROWS, PLAN_BAND, PLAN_HYBRID = 0, 1, 2, 3, 4
 
@@ -73,6 +73,7 @@ _p = ctypes.c_void_p
 _i32, _i64, _u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
 _int = ctypes.c_int
 _pi32 = ctypes.POINTER(ctypes.c_int32)
+_pi64 = ctypes.POINTER(ctypes.c_int64)
 _pf32 = ctypes.POINTER(ctypes.c_float)
 _pp = ctypes.POINTER(ctypes.c_void_p)
 
@@ -109,6 +110,15 @@ PROTOTYPES = {
     "vcsrmc_spmm": (_int, [_p, _p, _int, _i64, _i32, _i32, _p, _i64, _int, _p]),
     "vcsrmc_spmm_ex": (_int, [_p, _p, _int, _i64, _i32, _i32, _p, _i64, _int, _int, _p]),
     "vcsrmc_spmm_timed": (_int, [_p, _p, _int, _i64, _i32, _i32, _p, _i64, _int, _p, _pf32]),
+    "vcsrmc_mx_quantize": (_int, [_p, _int, _i64, _i64, _i32, _int, _p, _i64, _p, _i64, _p]),
+    "vcsrmc_mx_dequantize": (_int, [_p, _int, _i64, _p, _i64, _i64, _i32, _p, _int, _i64, _p]),
+    "vcsrmc_spmm_mx_workspace": (_int, [_p, _i32, _pi64]),
+    "vcsrmc_spmm_mx": (_int, [_p, _p, _int, _i64, _p, _i64, _i32, _p, _i64, _int, _p, _i64, _p]),
+    "vcsrmc_add_rms_norm": (_int, [_p, _int, _i64, _p, _i64, _p, _i64, _int, _p, _int, ctypes.c_float, _i64, _i32, _int,
+                                   _p, _i64, _p, _i64, _p, _p]),
+    "vcsrmc_add_rms_norm_backward_workspace": (_int, [_i64, _i32, _pi64]),
+    "vcsrmc_add_rms_norm_backward": (_int, [_p, _int, _i64, _p, _i64, _p, _i64, _int, _p, _int, _p, _i64, _i32, _p, _i64,
+                                            _p, _p, _i64, _p]),
     "vcsrmc_gen_csr": (_int, [_int, _i32, _u64, _int, _pp]),
     "vcsrmc_gen_dense_host": (_int, [_i64, _i32, _u64, _p, _int]),
     "vcsrmc_gen_dense_device": (_int, [_i64, _i32, _u64, _int, _p, _i64, _p]),

@@ -20,7 +20,8 @@ from typing import Optional
 import numpy as np
 
 from . import _lib
-from ._lib import F16, F32, PLAN_AUTO, PLAN_BAND, PLAN_HYBRID, PLAN_ROWS, PLAN_SEGMENT, VcsrmcError, call
+from ._lib import (BF16, F16, F32, MXF4, MXF8, PLAN_AUTO, PLAN_BAND, PLAN_HYBRID, PLAN_ROWS, PLAN_SEGMENT, VcsrmcError,
+                   call)
 
 
 def _ptr(a: np.ndarray) -> ctypes.c_void_p:
@@ -311,12 +312,258 @@ def _check_dense(B, C, O):
 
 def spmm(dV: DeviceVCSRMC, B, C, tileK: int = 128, accumulate: bool = False, stream=None, O: Optional[int] = None,
          plan: int = PLAN_AUTO):
-    """C[:, :O] (+)= A * B[:, :O] on the GPU, asynchronous on `stream` (default: torch's current)."""
+    """C[:, :O] (+)= A * B[:, :O] on the GPU, asynchronous on `stream` (default: torch's current).
+    B: a float16 or float32 tensor, or an MXDense (ROWS plan; the same call gives the same bits)."""
+    if isinstance(B, MXDense):
+        return _spmm_mx(dV, B, C, tileK, accumulate, stream, O, plan)
     O = int(B.shape[1]) if O is None else O
     _check_dense(B, C, O)
     call("vcsrmc_spmm_ex", dV.handle, ctypes.c_void_p(B.data_ptr()), _b_args(B), B.stride(0), O, tileK,
          ctypes.c_void_p(C.data_ptr()), C.stride(0), 1 if accumulate else 0, plan, _stream_handle(stream))
     return C
+
+
+MX_BLOCK = 32  # columns of an MX matrix that share a scale
+
+
+def _invalid(message: str) -> VcsrmcError:
+    return VcsrmcError(_lib.INVALID_ARG, message)
+
+
+class MXDense:
+    """A microscaled (MX) matrix on one GPU: elements and one power-of-two scale per 32 columns of a row.
+
+    data:  float8_e4m3fn [rows, cols] (MXF8), or uint8 [rows, ceil(cols / 2)] with two E2M1 elements per
+           byte, the even column in the low half (MXF4)
+    scale: float8_e8m0fnu (or uint8) [rows, ceil(cols / 32)]
+    Rows may be strided; columns may not. `cols` is needed for an odd number of MXF4 columns."""
+
+    def __init__(self, data, scale, cols: Optional[int] = None):
+        import torch
+        if not (isinstance(data, torch.Tensor) and isinstance(scale, torch.Tensor)) or data.dim() != 2 or scale.dim() != 2:
+            raise _invalid("MX elements and scales must be 2-D tensors")
+        if data.dtype == torch.float8_e4m3fn:
+            self.kind, per_byte = MXF8, 1
+        elif data.dtype == torch.uint8:
+            self.kind, per_byte = MXF4, 2
+        else:
+            raise _invalid(f"MX elements must be float8_e4m3fn (MXF8) or uint8 (MXF4), got {data.dtype}")
+        if scale.dtype not in (torch.float8_e8m0fnu, torch.uint8):
+            raise _invalid(f"MX scales must be float8_e8m0fnu or uint8, got {scale.dtype}")
+        self.rows, self.cols = int(data.shape[0]), int(data.shape[1]) * per_byte if cols is None else int(cols)
+        if self.cols < 0 or data.shape[1] < -(-self.cols // per_byte) or scale.shape[1] < -(-self.cols // MX_BLOCK) \
+                or scale.shape[0] != self.rows:
+            raise _invalid("MX elements and scales must hold every row and column")
+        if (data.stride(1) != 1 and data.shape[1] > 1) or (scale.stride(1) != 1 and scale.shape[1] > 1):
+            raise _invalid("the columns of MX elements and scales must be contiguous")
+        if data.device != scale.device:
+            raise _invalid("MX elements and scales must be on the same device")
+        self.data, self.scale = data, scale
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    def _args(self):
+        """Pointer, type, row stride, scale pointer and scale row stride, as the C ABI takes them."""
+        return (self.data.data_ptr(), self.kind, _row_stride(self.data), self.scale.data_ptr(), _row_stride(self.scale))
+
+    @staticmethod
+    def empty(rows: int, cols: int, kind: int = MXF8, device=None) -> "MXDense":
+        import torch
+        if kind not in (MXF8, MXF4):
+            raise _invalid("the microscaled kind must be MXF8 or MXF4")
+        data = torch.empty((rows, cols) if kind == MXF8 else (rows, (cols + 1) // 2), device=device,
+                           dtype=torch.float8_e4m3fn if kind == MXF8 else torch.uint8)
+        return MXDense(data, torch.empty((rows, -(-cols // MX_BLOCK)), dtype=torch.float8_e8m0fnu, device=device), cols)
+
+
+def _row_stride(t) -> int:
+    """Row stride of a 2-D tensor in elements; torch leaves the stride of a single row open."""
+    return int(t.stride(0)) if t.shape[0] > 1 else max(int(t.shape[1]), 1)
+
+
+def _dense_dtype(t, what: str) -> int:
+    import torch
+    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+    if code is None:
+        raise _invalid(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _dense_2d(t, what: str, device=None, shape=None, dtype=None):
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise _invalid(f"{what} must be a 2-D CUDA tensor with contiguous columns")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise _invalid(f"the rows of {what} must not overlap")
+    if device is not None and t.device != device:
+        raise _invalid(f"{what} must be on {device}, with the other tensors")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise _invalid(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise _invalid(f"{what} must be {dtype}, got {t.dtype}")
+    return t
+
+
+def _vector(t, what: str, device, n: int, dtype=None):
+    import torch
+    if not isinstance(t, torch.Tensor) or t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise _invalid(f"{what} must be a contiguous tensor of {n} values on {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise _invalid(f"{what} must be {dtype}, got {t.dtype}")
+    return t
+
+
+class _on:
+    """Makes `device` and `stream` (None: torch's current one there) current for the block, so that what it allocates belongs to the
+    stream that uses it; `.handle` is the stream for the C ABI."""
+
+    def __init__(self, device, stream):
+        import torch
+        if device.type != "cuda":
+            raise _invalid("microscaled operators run on CUDA tensors")
+        self.guard = None
+        if stream is None:
+            if torch.cuda.current_device() != device.index:
+                self.guard = torch.cuda.device(device)
+            self.handle = torch.cuda.current_stream(device).cuda_stream
+        else:
+            if not isinstance(stream, torch.cuda.Stream):
+                raw = int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
+                stream = torch.cuda.ExternalStream(raw, device=device)
+            if stream.device != device:
+                raise _invalid(f"the stream must be on {device}, with the tensors")
+            self.guard = torch.cuda.stream(stream)
+            self.handle = stream.cuda_stream
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _workspace(name: str, device, *args):
+    """The workspace a call asks for (of torch's allocator, on the current stream), and its size."""
+    import torch
+    n = ctypes.c_int64()
+    call(name, *args, ctypes.byref(n))
+    return (torch.empty(n.value, dtype=torch.uint8, device=device), n.value) if n.value else (None, 0)
+
+
+def _spmm_mx(dV: DeviceVCSRMC, B: MXDense, C, tileK: int, accumulate: bool, stream, O: Optional[int], plan: int):
+    import torch
+    O = B.cols if O is None else O
+    _dense_2d(C, "C", dtype=torch.float32)
+    if B.device != C.device or C.device.index != dV.device:
+        raise _invalid("A, B and C must be on the same device")
+    if plan not in (PLAN_AUTO, PLAN_ROWS):
+        raise _invalid("a microscaled B runs on the ROWS plan")
+    if tileK not in (16, 32, 64, 128, 256):
+        raise _invalid("tileK must be one of 16, 32, 64, 128, 256")
+    if B.cols < O or C.shape[1] < O or B.rows < dV.N or C.shape[0] < dV.M:
+        raise _invalid("B and C must hold A's columns and rows, with >= O columns")
+    with _on(C.device, stream) as on:
+        ws, n = _workspace("vcsrmc_spmm_mx_workspace", C.device, dV.handle, O)
+        call("vcsrmc_spmm_mx", dV.handle, *B._args(), O, C.data_ptr(), _row_stride(C), 1 if accumulate else 0,
+             None if ws is None else ws.data_ptr(), n, on.handle)
+    return C
+
+
+def mx_quantize(X, kind: int = MXF8, out: Optional[MXDense] = None, stream=None) -> MXDense:
+    """X (float32, float16 or bfloat16) in 8 (MXF8) or 4 bits (MXF4): the scale of 32 columns is the smallest power of two
+    under which their largest magnitude fits the element type; elements are rounded to nearest, ties to even."""
+    _dense_2d(X, "X")
+    rows, cols = X.shape
+    x_dtype = _dense_dtype(X, "X")
+    with _on(X.device, stream) as on:
+        if out is None:
+            out = MXDense.empty(rows, cols, kind, X.device)
+        elif out.kind != kind or out.shape != (rows, cols) or out.device != X.device:
+            raise _invalid("out must have X's shape and device, and the kind that is asked for")
+        q, q_dtype, ldq, s, lds = out._args()
+        call("vcsrmc_mx_quantize", X.data_ptr(), x_dtype, _row_stride(X), rows, cols, q_dtype, q, ldq, s, lds, on.handle)
+    return out
+
+
+def mx_dequantize(Q: MXDense, dtype=None, out=None, stream=None):
+    """The values an MXDense stands for, rounded to `dtype` (default float32)."""
+    import torch
+    with _on(Q.device, stream) as on:
+        if out is None:
+            out = torch.empty(Q.shape, dtype=torch.float32 if dtype is None else dtype, device=Q.device)
+        _dense_2d(out, "out", Q.device, Q.shape, dtype)
+        y_dtype = _dense_dtype(out, "out")
+        call("vcsrmc_mx_dequantize", *Q._args(), Q.rows, Q.cols, out.data_ptr(), y_dtype, _row_stride(out), on.handle)
+    return out
+
+
+def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, out: Optional[MXDense] = None, residual_out=None,
+                 stream=None):
+    """(Q, residual_out, inv_rms): s = X + residual, rounded to the residual's type (residual_out); inv_rms = 1 / sqrt(mean(s^2) +
+    eps) of every row (float32); Q = MX(s * inv_rms * weight). The residual has X's type, or X is float32 (a product's C). Without a
+    residual s is X, which is then returned in residual_out's place. residual_out may be the residual, or X of the same type (in place)."""
+    import torch
+    _dense_2d(X, "X")
+    rows, cols = X.shape
+    x_dtype, w_dtype = _dense_dtype(X, "X"), _dense_dtype(weight, "weight")
+    _vector(weight, "weight", X.device, cols)
+    if residual is not None:
+        _dense_2d(residual, "residual", X.device, X.shape)
+    r_type = X.dtype if residual is None else residual.dtype
+    r_dtype = x_dtype if residual is None else _dense_dtype(residual, "residual")
+    with _on(X.device, stream) as on:
+        if residual_out is not None:
+            _dense_2d(residual_out, "residual_out", X.device, X.shape, r_type)
+        elif residual is not None:
+            residual_out = torch.empty((rows, cols), dtype=r_type, device=X.device)
+        if out is None:
+            out = MXDense.empty(rows, cols, kind, X.device)
+        elif out.kind != kind or out.shape != (rows, cols) or out.device != X.device:
+            raise _invalid("out must have X's shape and device, and the kind that is asked for")
+        inv_rms = torch.empty(rows, dtype=torch.float32, device=X.device)
+        q, q_dtype, ldq, s, lds = out._args()
+        call("vcsrmc_add_rms_norm", X.data_ptr(), x_dtype, _row_stride(X),
+             None if residual is None else residual.data_ptr(), 0 if residual is None else _row_stride(residual),
+             None if residual_out is None else residual_out.data_ptr(), 0 if residual_out is None else _row_stride(residual_out), r_dtype,
+             weight.data_ptr(), w_dtype, eps, rows, cols, q_dtype, q, ldq, s, lds, inv_rms.data_ptr(), on.handle)
+    return out, X if residual_out is None else residual_out, inv_rms
+
+
+def add_rms_norm_backward(dY, weight, hidden, inv_rms, d_residual=None, out=None, stream=None):
+    """(dX, dweight) of add_rms_norm: dY is the gradient of the values Q stands for (float32 or hidden's type; the elements' rounding
+    counts as the identity), hidden and inv_rms are what the forward call returned, d_residual the gradient of its residual_out. dX, in
+    hidden's type, is the gradient of X and of the residual; dweight is float32. out (dX) may be d_residual, or dY of the same type."""
+    import torch
+    _dense_2d(dY, "dY")
+    rows, cols = dY.shape
+    dy_dtype, w_dtype = _dense_dtype(dY, "dY"), _dense_dtype(weight, "weight")
+    _vector(weight, "weight", dY.device, cols)
+    _dense_2d(hidden, "hidden", dY.device, dY.shape)
+    _vector(inv_rms, "inv_rms", dY.device, rows, torch.float32)
+    r_dtype = _dense_dtype(hidden, "hidden")
+    if d_residual is not None:
+        _dense_2d(d_residual, "d_residual", dY.device, dY.shape, hidden.dtype)
+    with _on(dY.device, stream) as on:
+        if out is None:
+            out = torch.empty((rows, cols), dtype=hidden.dtype, device=dY.device)
+        _dense_2d(out, "out", dY.device, dY.shape, hidden.dtype)
+        dweight = torch.empty(cols, dtype=torch.float32, device=dY.device)
+        ws, n = _workspace("vcsrmc_add_rms_norm_backward_workspace", dY.device, rows, cols)
+        call("vcsrmc_add_rms_norm_backward", dY.data_ptr(), dy_dtype, _row_stride(dY),
+             None if d_residual is None else d_residual.data_ptr(), 0 if d_residual is None else _row_stride(d_residual),
+             hidden.data_ptr(), _row_stride(hidden), r_dtype, weight.data_ptr(), w_dtype, inv_rms.data_ptr(), rows, cols,
+             out.data_ptr(), _row_stride(out), dweight.data_ptr(), None if ws is None else ws.data_ptr(), n, on.handle)
+    return out, dweight
 
 
 def run_vcsr_mc_spmm_gpu(dV: DeviceVCSRMC, B, O: int, tileK: int, C, stream=None, accumulate: bool = True) -> float:

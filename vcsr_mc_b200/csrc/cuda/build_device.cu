@@ -597,6 +597,7 @@ RowsLayout build_rows_layout(const int* row_ptr, const int* col, const float* va
     R.vals = vals.release();
     R.units = units.release();
     R.n_units = n_units;
+    R.n_chunks = count_chunks(hunits);
     R.split_rows = split.release();
     R.n_split_rows = int(n_split);
     return R;

@@ -27,7 +27,7 @@ struct RowsLayout {
     int* cols = nullptr;
     void* vals = nullptr;  // __half (FP16 format) or float
     int4* units = nullptr;
-    int64_t n_units = 0;
+    int64_t n_units = 0, n_chunks = 0;
     int* split_rows = nullptr;
     int n_split_rows = 0;
 };

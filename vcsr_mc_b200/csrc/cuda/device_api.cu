@@ -27,6 +27,7 @@
 #include "../host/parallel.hpp"
 #include "common.cuh"
 #include "build_device.hpp"
+#include "mx.hpp"
 #include "plan_band.hpp"
 #include "plan_rows.hpp"
 #include "spmm_launch.hpp"
@@ -47,7 +48,7 @@ struct vcsrmc_device_format {
     // ROWS plan
     bool has_rows = false;
     int4* units = nullptr;
-    int64_t n_units = 0;
+    int64_t n_units = 0, n_chunks = 0;
     int* rp = nullptr;
     int* cols = nullptr;
     void* rvals = nullptr;
@@ -569,6 +570,7 @@ VCSRMC_EXPORT int vcsrmc_upload_opts(const vcsrmc_format* f, int device, const v
                 static_assert(sizeof(dev::RowViewHost::Unit) == sizeof(int4), "unit layout");
                 d->units = reinterpret_cast<int4*>(upload_array(rv.units.data(), rv.units.size(), st));
                 d->n_units = int64_t(rv.units.size());
+                d->n_chunks = dev::count_chunks(rv.units);
                 d->split_rows = upload_array(rv.split_rows.data(), rv.split_rows.size(), st);
                 d->n_split_rows = int(rv.split_rows.size());
                 d->unit_nnz = unit_nnz;
@@ -809,6 +811,7 @@ VCSRMC_EXPORT int vcsrmc_build_device(int32_t M, int32_t N, int64_t nnz, const i
                 d->rvals = rows.vals;
                 d->units = rows.units;
                 d->n_units = rows.n_units;
+                d->n_chunks = rows.n_chunks;
                 d->split_rows = rows.split_rows;
                 d->n_split_rows = rows.n_split_rows;
                 d->unit_nnz = unit_nnz;
@@ -945,5 +948,204 @@ VCSRMC_EXPORT int vcsrmc_half_scale_device(const float* val, int64_t nnz, void* 
         static std::mutex scratch_mu;  // one scratch word per device: calls do not overlap
         std::lock_guard<std::mutex> lock(scratch_mu);
         *scale = half_scale_from_absmax(dev::device_abs_max_noalloc(val, nnz, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+// ---- microscaled (MX) dense operands ---------------------------------------------------------------
+namespace {
+
+constexpr int32_t kMxMaxO = 1 << 30;        // columns of a quantised or normalised matrix
+constexpr int32_t kMxMaxSpmmO = 65535 * 128;  // columns of one product (a grid's y extent of 128-column slabs)
+
+[[noreturn]] void invalid(const std::string& what) { throw StatusError(VCSRMC_INVALID_ARG, what); }
+
+int dense_bytes(int dtype, const char* what) {
+    if (dtype == VCSRMC_F32) return 4;
+    if (dtype == VCSRMC_F16 || dtype == VCSRMC_BF16) return 2;
+    invalid(std::string(what) + " must be fp32, fp16 or bf16");
+}
+
+void check_shape(int64_t rows, int32_t O) {
+    if (rows < 0) invalid("rows must be >= 0");
+    if (O < 1 || O > kMxMaxO) invalid("O must be in [1, 2^30]");
+}
+
+dev::DenseView dense_view(const void* p, int dtype, int64_t ld, int64_t rows, int32_t O, const char* what) {
+    const int bytes = dense_bytes(dtype, what);
+    if (rows > 0 && !p) invalid(std::string("NULL ") + what);
+    if (reinterpret_cast<uintptr_t>(p) % uintptr_t(bytes)) invalid(std::string(what) + " is not aligned to its element type");
+    if (ld < O) invalid(std::string(what) + " needs a row stride of at least O elements");
+    dev::DenseView v;
+    v.p = const_cast<void*>(p);
+    v.dtype = dtype;
+    v.ld = ld;
+    return v;
+}
+
+dev::MxView mx_view(const void* Q, int q_dtype, int64_t ldq, const uint8_t* S, int64_t lds, int64_t rows, int32_t O) {
+    if (q_dtype != VCSRMC_MXF8 && q_dtype != VCSRMC_MXF4) invalid("the microscaled type must be VCSRMC_MXF8 or VCSRMC_MXF4");
+    if (rows > 0 && (!Q || !S)) invalid("NULL elements or scales");
+    const int64_t row_bytes = q_dtype == VCSRMC_MXF4 ? (int64_t(O) + 1) / 2 : O;
+    if (ldq < row_bytes) invalid("ldq must cover a row's elements, in bytes");
+    if (lds < (int64_t(O) + 31) / 32) invalid("lds must cover a row's scales, one for every 32 columns");
+    dev::MxView v;
+    v.q = static_cast<uint8_t*>(const_cast<void*>(Q));
+    v.ldq = ldq;
+    v.s = const_cast<uint8_t*>(S);
+    v.lds = lds;
+    v.q4 = q_dtype == VCSRMC_MXF4;
+    return v;
+}
+
+void check_weight(const void* w, int w_dtype) {
+    const int bytes = dense_bytes(w_dtype, "weight");
+    if (!w) invalid("NULL weight");
+    if (reinterpret_cast<uintptr_t>(w) % uintptr_t(bytes)) invalid("weight is not aligned to its element type");
+}
+
+int sm_count() {
+    int device = 0, sms = 0;
+    cuda_check(cudaGetDevice(&device), "cudaGetDevice");
+    cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "cudaDeviceGetAttribute");
+    return sms;
+}
+
+int64_t spmm_mx_bytes(const vcsrmc_device_format* d, int32_t O) { return d->n_chunks * int64_t(O) * int64_t(sizeof(float)); }
+
+void check_spmm_mx(const vcsrmc_device_format* d, int32_t O) {
+    if (!d) invalid("NULL format");
+    if (O < 1 || O > kMxMaxSpmmO) invalid("O must be in [1, 8388480]");
+    if (!d->has_rows) invalid("a microscaled B runs on the ROWS plan, whose layout was not uploaded");
+}
+
+}  // namespace
+
+VCSRMC_EXPORT int vcsrmc_mx_quantize(const void* X, int x_dtype, int64_t ldx, int64_t rows, int32_t O, int q_dtype, void* Q, int64_t ldq,
+                                     uint8_t* S, int64_t lds, void* stream) {
+    return guarded([&] {
+        check_shape(rows, O);
+        const dev::DenseView x = dense_view(X, x_dtype, ldx, rows, O, "X");
+        const dev::MxView q = mx_view(Q, q_dtype, ldq, S, lds, rows, O);
+        cuda_check(dev::mx_quantize(x, rows, O, q, static_cast<cudaStream_t>(stream)), "mx_quantize");
+    });
+}
+
+VCSRMC_EXPORT int vcsrmc_mx_dequantize(const void* Q, int q_dtype, int64_t ldq, const uint8_t* S, int64_t lds, int64_t rows, int32_t O,
+                                       void* Y, int y_dtype, int64_t ldy, void* stream) {
+    return guarded([&] {
+        check_shape(rows, O);
+        const dev::DenseView y = dense_view(Y, y_dtype, ldy, rows, O, "Y");
+        const dev::MxView q = mx_view(Q, q_dtype, ldq, S, lds, rows, O);
+        cuda_check(dev::mx_dequantize(q, rows, O, y, static_cast<cudaStream_t>(stream)), "mx_dequantize");
+    });
+}
+
+VCSRMC_EXPORT int vcsrmc_spmm_mx_workspace(const vcsrmc_device_format* d, int32_t O, int64_t* bytes) {
+    return guarded([&] {
+        check_spmm_mx(d, O);
+        if (!bytes) invalid("NULL bytes");
+        *bytes = spmm_mx_bytes(d, O);
+    });
+}
+
+VCSRMC_EXPORT int vcsrmc_spmm_mx(const vcsrmc_device_format* d, const void* Q, int q_dtype, int64_t ldq, const uint8_t* S, int64_t lds,
+                                 int32_t O, float* C, int64_t ldc, int accumulate, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+    return guarded([&] {
+        check_spmm_mx(d, O);
+        const dev::MxView q = mx_view(Q, q_dtype, ldq, S, lds, d->N, O);
+        const dev::DenseView c = dense_view(C, VCSRMC_F32, ldc, d->M, O, "C");
+        if (ldq > INT32_MAX || lds > INT32_MAX) invalid("ldq and lds must fit 31 bits");
+        const int64_t need = spmm_mx_bytes(d, O);
+        if (need > 0 && (!workspace || workspace_bytes < need))
+            invalid("the workspace is smaller than vcsrmc_spmm_mx_workspace says: " + std::to_string(need) + " bytes");
+        if (reinterpret_cast<uintptr_t>(workspace) % 16) invalid("the workspace must be 16-byte aligned");
+        DeviceGuard guard(d->device);
+        dev::RowPlanView P;
+        P.units = d->units;
+        P.n_units = d->n_units;
+        P.rp = d->rp;
+        P.cols = d->cols;
+        P.vals = d->rvals;
+        P.vals_f16 = d->fp32 ? 0 : 1;
+        P.split_rows = d->split_rows;
+        P.n_split_rows = d->n_split_rows;
+        P.n_chunks = d->n_chunks;
+        P.M = d->M;
+        P.N = d->N;
+        P.scale = d->scale;
+        P.hot.hot_cols = d->hot_cols;
+        cuda_check(dev::spmm_rows_mx(P, q, O, static_cast<float*>(c.p), ldc, accumulate != 0, static_cast<float*>(workspace),
+                                     static_cast<cudaStream_t>(stream)),
+                   "SpMM launch (rows plan, microscaled B)");
+    });
+}
+
+VCSRMC_EXPORT int vcsrmc_add_rms_norm(const void* X, int x_dtype, int64_t ldx, const void* residual, int64_t ldr, void* residual_out,
+                                      int64_t ldo, int r_dtype, const void* weight, int w_dtype, float eps, int64_t rows, int32_t O,
+                                      int q_dtype, void* Q, int64_t ldq, uint8_t* S, int64_t lds, float* inv_rms, void* stream) {
+    return guarded([&] {
+        check_shape(rows, O);
+        dev::RmsNormArgs a;
+        a.x = dense_view(X, x_dtype, ldx, rows, O, "X");
+        if (x_dtype != VCSRMC_F32 && r_dtype != x_dtype) invalid("the residual has X's type, or X is fp32");
+        a.residual = dense_view(residual, r_dtype, residual ? ldr : O, residual ? rows : 0, O, "residual");
+        a.residual_out = dense_view(residual_out, r_dtype, residual_out ? ldo : O, residual_out ? rows : 0, O, "residual_out");
+        check_weight(weight, w_dtype);
+        if (!(eps >= 0.f) || eps > 3.4e38f) invalid("eps must be finite and not negative");
+        a.weight = weight;
+        a.w_dtype = w_dtype;
+        a.eps = eps;
+        a.rows = rows;
+        a.O = O;
+        a.out = mx_view(Q, q_dtype, ldq, S, lds, rows, O);
+        if (reinterpret_cast<uintptr_t>(inv_rms) % 4) invalid("inv_rms is not aligned to its element type");
+        a.inv_rms = inv_rms;
+        if (rows > 0) cuda_check(dev::add_rms_norm(a, static_cast<cudaStream_t>(stream)), "add_rms_norm");
+    });
+}
+
+VCSRMC_EXPORT int vcsrmc_add_rms_norm_backward_workspace(int64_t rows, int32_t O, int64_t* bytes) {
+    return guarded([&] {
+        check_shape(rows, O);
+        if (!bytes) invalid("NULL bytes");
+        *bytes = rows == 0 ? 0 : dev::rms_norm_grad_workspace(rows, O, sm_count());
+    });
+}
+
+VCSRMC_EXPORT int vcsrmc_add_rms_norm_backward(const void* dY, int dy_dtype, int64_t lddy, const void* d_residual, int64_t lddr,
+                                               const void* hidden, int64_t ldh, int r_dtype, const void* weight, int w_dtype,
+                                               const float* inv_rms, int64_t rows, int32_t O, void* dX, int64_t lddx, float* dweight,
+                                               void* workspace, int64_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        check_shape(rows, O);
+        dev::RmsNormGradArgs a;
+        a.dy = dense_view(dY, dy_dtype, lddy, rows, O, "dY");
+        if (dy_dtype != VCSRMC_F32 && r_dtype != dy_dtype) invalid("the residual's gradient has dY's type, or dY is fp32");
+        a.d_residual = dense_view(d_residual, r_dtype, d_residual ? lddr : O, d_residual ? rows : 0, O, "d_residual");
+        a.hidden = dense_view(hidden, r_dtype, ldh, rows, O, "hidden");
+        a.dx = dense_view(dX, r_dtype, lddx, rows, O, "dX");
+        check_weight(weight, w_dtype);
+        a.weight = weight;
+        a.w_dtype = w_dtype;
+        if ((rows > 0 && !inv_rms) || !dweight) invalid("NULL inv_rms or dweight");
+        if (reinterpret_cast<uintptr_t>(inv_rms) % 4 || reinterpret_cast<uintptr_t>(dweight) % 4)
+            invalid("inv_rms and dweight must be aligned to their element type");
+        a.inv_rms = inv_rms;
+        a.rows = rows;
+        a.O = O;
+        a.dweight = dweight;
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (rows == 0) {
+            cuda_check(cudaMemsetAsync(dweight, 0, sizeof(float) * size_t(O), st), "cudaMemsetAsync");
+            return;
+        }
+        const int sms = sm_count();
+        const int64_t need = dev::rms_norm_grad_workspace(rows, O, sms);
+        if (!workspace || workspace_bytes < need)
+            invalid("the workspace is smaller than vcsrmc_add_rms_norm_backward_workspace says: " + std::to_string(need) + " bytes");
+        if (reinterpret_cast<uintptr_t>(workspace) % 16) invalid("the workspace must be 16-byte aligned");
+        a.workspace = static_cast<float*>(workspace);
+        cuda_check(dev::add_rms_norm_backward(a, sms, st), "add_rms_norm_backward");
     });
 }

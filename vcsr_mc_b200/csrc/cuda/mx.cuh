@@ -1,0 +1,166 @@
+// Microscaled (MX) elements: 32 consecutive columns of a row share one power-of-two scale.
+//   element  E4M3 (8 bits, largest 448 = 1.75 * 2^8) or E2M1 (4 bits, largest 6 = 1.5 * 2^2)
+//   scale    E8M0, one byte: 2^(code - 127), 255 = NaN
+// The scale is the smallest power of two (from 2^-127) under which the block's largest magnitude
+// fits the element type, so no element is clipped; x * 2^-e is exact (a power of two) but for results
+// below fp32's normal range, which round to zero anyway, and the one rounding is the element's, to
+// nearest with ties to even. A block that holds an infinity or a NaN gets scale 255 and zero elements.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace vcsrmc {
+namespace dev {
+
+constexpr int kMxBlock = 32;       // columns per scale
+constexpr uint32_t kMxNan = 255u;  // scale code of a block with an infinity or a NaN
+
+// Scale code of a block from the bits of its largest |x| (a NaN's bits are above infinity's).
+__device__ __forceinline__ uint32_t mx_scale_code(uint32_t amax_bits, bool q4) {
+    if (amax_bits >= 0x7f800000u) return kMxNan;
+    const int k = int(amax_bits >> 23);  // amax = 1.m * 2^(k - 127); a subnormal (k = 0) clamps to code 0
+    const uint32_t m = amax_bits & 0x7fffffu;
+    const int code = q4 ? k - 2 + (m > 0x400000u) : k - 8 + (m > 0x600000u);
+    return uint32_t(max(code, 0));
+}
+// 2^-e of a finite block's code (codes reach 253 at most, so this is a normal number).
+__device__ __forceinline__ float mx_inverse_scale(uint32_t code) { return __uint_as_float((254u - code) << 23); }
+// 2^(code - 127); code 0 is subnormal, code 255 NaN.
+__device__ __forceinline__ float mx_scale_value(uint32_t code) {
+    const uint32_t bits = code == 0 ? 0x00400000u : code << 23;
+    return __uint_as_float(code == kMxNan ? 0x7fffffffu : bits);
+}
+
+// Two elements, `lo` in the low half of the result (8 bits of it for E2M1, 16 for E4M3).
+__device__ __forceinline__ uint32_t mx_encode2_e2m1(float lo, float hi) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ uint32_t mx_encode2_e4m3(float lo, float hi) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+// Two elements as f16x2 (exact), the low half of the input first.
+__device__ __forceinline__ uint32_t mx_decode2_e2m1(uint32_t byte) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(r) : "r"(byte));
+    return r;
+}
+__device__ __forceinline__ uint32_t mx_decode2_e4m3(uint32_t half) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)half));
+    return r;
+}
+__device__ __forceinline__ float2 mx_f16x2_to_f32(uint32_t h) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// ---- dense elements (fp32, fp16, bf16) ---------------------------------------------------------
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Eight consecutive elements; `vec`: p is 16-byte aligned and all eight exist, else the first nv are
+// read one by one and the others are 0.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int nv, bool vec, float (&v)[8]) {
+    if (vec && nv == 8) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const T* h = reinterpret_cast<const T*>(&w[i]);
+                v[2 * i] = to_f32(h[0]);
+                v[2 * i + 1] = to_f32(h[1]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < nv ? to_f32(p[i]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int nv, bool vec, const float (&v)[8]) {
+    if (vec && nv == 8) {
+        if constexpr (sizeof(T) == 4) {
+            __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+            __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                T* h = reinterpret_cast<T*>(&w[i]);
+                h[0] = from_f32<T>(v[2 * i]);
+                h[1] = from_f32<T>(v[2 * i + 1]);
+            }
+            __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < nv) p[i] = from_f32<T>(v[i]);
+    }
+}
+
+// Quantises and stores eight columns of a block held by four neighbouring lanes (8 columns each; all
+// 32 lanes of the warp take part). `q` is the eight columns' place in the row (byte c for E4M3, c / 2 for
+// E2M1), `s` the block's scale; nv of the eight columns exist (0: nothing is stored). `vec`: q is
+// aligned to its full store (8 bytes for E4M3, 4 for E2M1).
+__device__ __forceinline__ void mx_store_block(const float (&y)[8], int nv, bool q4, uint8_t* q, uint8_t* s, bool vec) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max(amax, i < nv ? __float_as_uint(y[i]) & 0x7fffffffu : 0u);
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t code = mx_scale_code(amax, q4);
+    const float inv = code == kMxNan ? 0.f : mx_inverse_scale(code);
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = code == kMxNan || i >= nv ? 0.f : y[i] * inv;
+    if (nv <= 0) return;
+    if ((threadIdx.x & 3) == 0) *s = uint8_t(code);
+    if (q4) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= mx_encode2_e2m1(t[2 * i], t[2 * i + 1]) << (8 * i);
+        if (vec && nv == 8) {
+            *reinterpret_cast<uint32_t*>(q) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (2 * i < nv) q[i] = uint8_t(w >> (8 * i));
+        }
+    } else {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = mx_encode2_e4m3(t[4 * i], t[4 * i + 1]) | (mx_encode2_e4m3(t[4 * i + 2], t[4 * i + 3]) << 16);
+        if (vec && nv == 8) {
+            *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < nv) q[i] = uint8_t(w[i >> 2] >> (8 * (i & 3)));
+        }
+    }
+}
+
+}  // namespace dev
+}  // namespace vcsrmc

@@ -1,0 +1,65 @@
+// Launchers of the microscaled (MX) operators: quantise, dequantise, residual addition with RMS norm
+// and its backward pass, and the rows plan with an MX operand (see mx.cuh for the format).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "plan_rows.hpp"
+
+namespace vcsrmc {
+namespace dev {
+
+// A strided row-major matrix of fp32, fp16 or bf16 (VCSRMC_F32, _F16, _BF16); ld in elements.
+struct DenseView {
+    void* p = nullptr;
+    int dtype = 0;
+    int64_t ld = 0;
+};
+
+// An MX matrix: element rows ldq bytes apart, scale rows lds bytes apart.
+struct MxView {
+    uint8_t* q = nullptr;
+    int64_t ldq = 0;
+    uint8_t* s = nullptr;
+    int64_t lds = 0;
+    bool q4 = false;
+};
+
+cudaError_t mx_quantize(const DenseView& X, int64_t rows, int O, const MxView& Q, cudaStream_t st);
+cudaError_t mx_dequantize(const MxView& Q, int64_t rows, int O, const DenseView& Y, cudaStream_t st);
+
+// s = round(x + residual) to residual_out's type; Q = MX(s * inv_rms * weight). residual.p and
+// residual_out.p and inv_rms may be null (no addition, nothing stored).
+struct RmsNormArgs {
+    DenseView x, residual, residual_out;
+    const void* weight = nullptr;
+    int w_dtype = 0;
+    float eps = 0.f;
+    int64_t rows = 0;
+    int O = 0;
+    MxView out;
+    float* inv_rms = nullptr;
+};
+cudaError_t add_rms_norm(const RmsNormArgs& a, cudaStream_t st);
+
+struct RmsNormGradArgs {
+    DenseView dy, d_residual, hidden, dx;
+    const void* weight = nullptr;
+    int w_dtype = 0;
+    const float* inv_rms = nullptr;
+    int64_t rows = 0;
+    int O = 0;
+    float* dweight = nullptr;
+    float* workspace = nullptr;  // rms_norm_grad_workspace(rows, O) bytes
+};
+int64_t rms_norm_grad_workspace(int64_t rows, int O, int sms);
+cudaError_t add_rms_norm_backward(const RmsNormGradArgs& a, int sms, cudaStream_t st);
+
+// C (+)= A * B with an MX operand B over the row view. `partial`: P.n_chunks * O floats (null when
+// P.n_chunks is 0), one row for every chunk of a split row; they are summed in chunk order.
+cudaError_t spmm_rows_mx(const RowPlanView& P, const MxView& B, int O, float* C, int64_t ldc, bool accumulate,
+                         float* partial, cudaStream_t st);
+
+}  // namespace dev
+}  // namespace vcsrmc

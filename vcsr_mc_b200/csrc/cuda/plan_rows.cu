@@ -681,6 +681,11 @@ void pack_units(const int* rp, int M, int unit_nnz, std::vector<RowViewHost::Uni
     }
 }
 
+int64_t count_chunks(const std::vector<RowViewHost::Unit>& units) {
+    const auto light = std::find_if(units.begin(), units.end(), [](const RowViewHost::Unit& u) { return u.y >= 0; });
+    return int64_t(light - units.begin());
+}
+
 RowViewHost build_row_view(const VCSRMC& v, int unit_nnz) {
     RowViewHost h;
     const int M = v.M;

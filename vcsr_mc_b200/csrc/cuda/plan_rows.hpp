@@ -32,6 +32,8 @@ RowViewHost build_row_view(const VCSRMC& v, int unit_nnz);
 // store; a run may still hold empty rows between non-empty ones).
 void pack_units(const int* rp, int M, int unit_nnz, std::vector<RowViewHost::Unit>& units,
                 std::vector<int>& split_rows, bool skip_empty = false);
+// Units that are chunks of split rows: they come first, in the order of their rows.
+int64_t count_chunks(const std::vector<RowViewHost::Unit>& units);
 // The unit size for a matrix of `nnz` entries on a GPU with `sms` SMs: the largest power of two
 // in [16, 256] that still gives every resident lane group (48 per SM) about four units.
 int choose_unit_nnz(int64_t nnz, int sms);
@@ -61,6 +63,7 @@ struct RowPlanView {
     int vals_f16;
     const int* split_rows;
     int n_split_rows;
+    int64_t n_chunks = 0;  // leading units that are chunks of split rows
     int M;
     int N = 0;  // columns of A (rows of B): bounds the B row offsets the kernel forms
     float scale;
