@@ -271,7 +271,7 @@ def test_product_scaled_format_hot_columns_and_extremes(cuda):
 
 
 def test_product_refusals(cuda):
-    M, N = 20, 30
+    M, N = 20, 130
     csr = sparse(M, N, 0.3, 5, long_row=1)
     dV = handle(M, N, *csr, False, rows_unit_nnz=16)
     codes, scales = features(N, 64, 1, "mxf8")
@@ -284,7 +284,7 @@ def test_product_refusals(cuda):
             call()
     from vcsr_mc_b200 import _lib
     with pytest.raises(vm.VcsrmcError):  # no workspace for the split row
-        _lib.call("vcsrmc_spmm_mx", dV.handle, *Q._args(), 64, C.data_ptr(), 64, 0, None, 0, None)
+        _lib.call("vcsrmc_spmm_mx", dV.handle, *Q._args, 64, C.data_ptr(), 64, 0, None, 0, None)
     only_segment = vm.upload_vcsr_mc_device(vm.csr_to_vcsr_mc(vm.CSR.from_arrays(M, N, *csr), segw=32), plans=[vm.PLAN_SEGMENT])
     with pytest.raises(vm.VcsrmcError):
         vm.spmm(only_segment, Q, C)

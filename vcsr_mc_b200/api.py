@@ -15,6 +15,7 @@ every computation runs in libvcsrmc.so.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import numpy as np
@@ -201,6 +202,7 @@ class DeviceVCSRMC:
     def __init__(self, handle: ctypes.c_void_p, host: Optional[VCSRMC], device: int, **shape):
         self._h = handle
         self.device = device
+        self._mx_workspace = {}
         if host is not None:
             shape = dict(M=host.M, N=host.N, fp32=host.fp32, scale=host.scale, segw=host.segw)
         self.M, self.N, self.fp32, self.scale, self.segw = (shape[k] for k in ("M", "N", "fp32", "scale", "segw"))
@@ -222,6 +224,15 @@ class DeviceVCSRMC:
     @property
     def handle(self) -> ctypes.c_void_p:
         return self._h
+
+    def mx_workspace(self, O: int) -> int:
+        """Bytes of workspace of a product with O columns of a microscaled B (vcsrmc_spmm_mx_workspace)."""
+        n = self._mx_workspace.get(O)
+        if n is None:
+            size = ctypes.c_int64()
+            call("vcsrmc_spmm_mx_workspace", self._h, O, ctypes.byref(size))
+            n = self._mx_workspace[O] = size.value
+        return n
 
     def free(self) -> None:
         h, self._h = self._h, None
@@ -338,133 +349,144 @@ class MXDense:
     scale: float8_e8m0fnu (or uint8) [rows, ceil(cols / 32)]
     Rows may be strided; columns may not. `cols` is needed for an odd number of MXF4 columns."""
 
+    __slots__ = ("data", "scale", "kind", "rows", "cols", "device", "_args")
+
     def __init__(self, data, scale, cols: Optional[int] = None):
         import torch
         if not (isinstance(data, torch.Tensor) and isinstance(scale, torch.Tensor)) or data.dim() != 2 or scale.dim() != 2:
             raise _invalid("MX elements and scales must be 2-D tensors")
         if data.dtype == torch.float8_e4m3fn:
-            self.kind, per_byte = MXF8, 1
+            kind, per_byte = MXF8, 1
         elif data.dtype == torch.uint8:
-            self.kind, per_byte = MXF4, 2
+            kind, per_byte = MXF4, 2
         else:
             raise _invalid(f"MX elements must be float8_e4m3fn (MXF8) or uint8 (MXF4), got {data.dtype}")
         if scale.dtype not in (torch.float8_e8m0fnu, torch.uint8):
             raise _invalid(f"MX scales must be float8_e8m0fnu or uint8, got {scale.dtype}")
-        self.rows, self.cols = int(data.shape[0]), int(data.shape[1]) * per_byte if cols is None else int(cols)
-        if self.cols < 0 or data.shape[1] < -(-self.cols // per_byte) or scale.shape[1] < -(-self.cols // MX_BLOCK) \
-                or scale.shape[0] != self.rows:
+        rows, cols = int(data.shape[0]), int(data.shape[1]) * per_byte if cols is None else int(cols)
+        if cols < 0 or data.shape[1] < -(-cols // per_byte) or scale.shape[1] < -(-cols // MX_BLOCK) or scale.shape[0] != rows:
             raise _invalid("MX elements and scales must hold every row and column")
         if (data.stride(1) != 1 and data.shape[1] > 1) or (scale.stride(1) != 1 and scale.shape[1] > 1):
             raise _invalid("the columns of MX elements and scales must be contiguous")
         if data.device != scale.device:
             raise _invalid("MX elements and scales must be on the same device")
-        self.data, self.scale = data, scale
+        self._set(data, scale, kind, rows, cols, data.device, _row_stride(data), _row_stride(scale))
 
-    @property
-    def device(self):
-        return self.data.device
+    def _set(self, data, scale, kind, rows, cols, device, ldq, lds):
+        self.data, self.scale, self.kind, self.rows, self.cols, self.device = data, scale, kind, rows, cols, device
+        # pointer, type, row stride, scale pointer and scale row stride, as the C ABI takes them
+        self._args = (data.data_ptr(), kind, ldq, scale.data_ptr(), lds)
 
     @property
     def shape(self):
         return (self.rows, self.cols)
 
-    def _args(self):
-        """Pointer, type, row stride, scale pointer and scale row stride, as the C ABI takes them."""
-        return (self.data.data_ptr(), self.kind, _row_stride(self.data), self.scale.data_ptr(), _row_stride(self.scale))
-
     @staticmethod
     def empty(rows: int, cols: int, kind: int = MXF8, device=None) -> "MXDense":
+        """An MXDense to write to. Its rows start at multiples of 16 bytes (8 columns of scales: 4), whatever `cols` is, so that
+        every operator can use its widest loads and stores."""
         import torch
         if kind not in (MXF8, MXF4):
             raise _invalid("the microscaled kind must be MXF8 or MXF4")
-        data = torch.empty((rows, cols) if kind == MXF8 else (rows, (cols + 1) // 2), device=device,
-                           dtype=torch.float8_e4m3fn if kind == MXF8 else torch.uint8)
-        return MXDense(data, torch.empty((rows, -(-cols // MX_BLOCK)), dtype=torch.float8_e8m0fnu, device=device), cols)
+        width, blocks = (cols if kind == MXF8 else (cols + 1) // 2), -(-cols // MX_BLOCK)
+        ldq, lds = -(-width // 16) * 16, -(-blocks // 4) * 4
+        data = torch.empty(rows, ldq, dtype=torch.float8_e4m3fn if kind == MXF8 else torch.uint8, device=device)
+        scale = torch.empty(rows, lds, dtype=torch.float8_e8m0fnu, device=device)
+        if ldq != width:
+            data = data[:, :width]
+        if lds != blocks:
+            scale = scale[:, :blocks]
+        out = MXDense.__new__(MXDense)
+        out._set(data, scale, kind, rows, cols, data.device, ldq, lds)
+        return out
 
 
 def _row_stride(t) -> int:
     """Row stride of a 2-D tensor in elements; torch leaves the stride of a single row open."""
-    return int(t.stride(0)) if t.shape[0] > 1 else max(int(t.shape[1]), 1)
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+_DENSE = None  # torch dtype -> VCSRMC code
 
 
 def _dense_dtype(t, what: str) -> int:
-    import torch
-    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+    global _DENSE
+    if _DENSE is None:
+        import torch
+        _DENSE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    code = _DENSE.get(getattr(t, "dtype", None))
     if code is None:
-        raise _invalid(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+        raise _invalid(f"{what} must be a float32, float16 or bfloat16 tensor")
     return code
 
 
 def _dense_2d(t, what: str, device=None, shape=None, dtype=None):
-    import torch
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise _invalid(f"{what} must be a 2-D CUDA tensor with contiguous columns")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    """Checks a dense matrix and returns (pointer, row stride)."""
+    shp = getattr(t, "shape", ())
+    if len(shp) != 2 or not t.is_cuda:
+        raise _invalid(f"{what} must be a 2-D CUDA tensor")
+    ld, step = t.stride()
+    if step != 1 and shp[1] > 1:
+        raise _invalid(f"the columns of {what} must be contiguous")
+    if shp[0] <= 1:
+        ld = max(shp[1], 1)
+    elif ld < shp[1]:
         raise _invalid(f"the rows of {what} must not overlap")
     if device is not None and t.device != device:
         raise _invalid(f"{what} must be on {device}, with the other tensors")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise _invalid(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if shape is not None and shp != shape:
+        raise _invalid(f"{what} must be {tuple(shape)}, got {tuple(shp)}")
     if dtype is not None and t.dtype != dtype:
         raise _invalid(f"{what} must be {dtype}, got {t.dtype}")
-    return t
+    return t.data_ptr(), ld
 
 
-def _vector(t, what: str, device, n: int, dtype=None):
-    import torch
-    if not isinstance(t, torch.Tensor) or t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous():
+def _vector(t, what: str, device, n: int, dtype=None) -> int:
+    """Checks a contiguous vector of n values and returns its pointer."""
+    if len(getattr(t, "shape", ())) != 1 or t.shape[0] != n or t.device != device or (n > 1 and t.stride(0) != 1):
         raise _invalid(f"{what} must be a contiguous tensor of {n} values on {device}")
     if dtype is not None and t.dtype != dtype:
         raise _invalid(f"{what} must be {dtype}, got {t.dtype}")
-    return t
+    return t.data_ptr()
 
 
-class _on:
-    """Makes `device` and `stream` (None: torch's current one there) current for the block, so that what it allocates belongs to the
-    stream that uses it; `.handle` is the stream for the C ABI."""
-
-    def __init__(self, device, stream):
-        import torch
-        if device.type != "cuda":
-            raise _invalid("microscaled operators run on CUDA tensors")
-        self.guard = None
-        if stream is None:
-            if torch.cuda.current_device() != device.index:
-                self.guard = torch.cuda.device(device)
-            self.handle = torch.cuda.current_stream(device).cuda_stream
-        else:
-            if not isinstance(stream, torch.cuda.Stream):
-                raw = int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
-                stream = torch.cuda.ExternalStream(raw, device=device)
-            if stream.device != device:
-                raise _invalid(f"the stream must be on {device}, with the tensors")
-            self.guard = torch.cuda.stream(stream)
-            self.handle = stream.cuda_stream
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
-
-
-def _workspace(name: str, device, *args):
-    """The workspace a call asks for (of torch's allocator, on the current stream), and its size."""
+def _on(device, stream):
+    """(guard, stream handle): the guard makes `device` and `stream` (None: torch's current one there) current, so that what is
+    allocated under it belongs to the stream that uses it; it is None where they are current already."""
     import torch
-    n = ctypes.c_int64()
-    call(name, *args, ctypes.byref(n))
-    return (torch.empty(n.value, dtype=torch.uint8, device=device), n.value) if n.value else (None, 0)
+    if device.type != "cuda":
+        raise _invalid("microscaled operators run on CUDA tensors")
+    if stream is None:
+        guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
+        return guard, torch._C._cuda_getCurrentRawStream(device.index)
+    if not isinstance(stream, torch.cuda.Stream):
+        raw = int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
+        stream = torch.cuda.ExternalStream(raw, device=device)
+    if stream.device != device:
+        raise _invalid(f"the stream must be on {device}, with the tensors")
+    return torch.cuda.stream(stream), stream.cuda_stream
+
+
+def _under(guard, fn):
+    if guard is None:
+        return fn()
+    with guard:
+        return fn()
+
+
+def _out_mx(out: Optional[MXDense], rows: int, cols: int, kind: int, device) -> MXDense:
+    if out is None:
+        return MXDense.empty(rows, cols, kind, device)
+    if out.kind != kind or out.rows != rows or out.cols != cols or out.device != device:
+        raise _invalid("out must have X's shape and device, and the kind that is asked for")
+    return out
 
 
 def _spmm_mx(dV: DeviceVCSRMC, B: MXDense, C, tileK: int, accumulate: bool, stream, O: Optional[int], plan: int):
     import torch
     O = B.cols if O is None else O
-    _dense_2d(C, "C", dtype=torch.float32)
-    if B.device != C.device or C.device.index != dV.device:
+    c, ldc = _dense_2d(C, "C", B.device, None, torch.float32)
+    if C.device.index != dV.device:
         raise _invalid("A, B and C must be on the same device")
     if plan not in (PLAN_AUTO, PLAN_ROWS):
         raise _invalid("a microscaled B runs on the ROWS plan")
@@ -472,39 +494,46 @@ def _spmm_mx(dV: DeviceVCSRMC, B: MXDense, C, tileK: int, accumulate: bool, stre
         raise _invalid("tileK must be one of 16, 32, 64, 128, 256")
     if B.cols < O or C.shape[1] < O or B.rows < dV.N or C.shape[0] < dV.M:
         raise _invalid("B and C must hold A's columns and rows, with >= O columns")
-    with _on(C.device, stream) as on:
-        ws, n = _workspace("vcsrmc_spmm_mx_workspace", C.device, dV.handle, O)
-        call("vcsrmc_spmm_mx", dV.handle, *B._args(), O, C.data_ptr(), _row_stride(C), 1 if accumulate else 0,
-             None if ws is None else ws.data_ptr(), n, on.handle)
+    guard, st = _on(C.device, stream)
+    n = dV.mx_workspace(O)
+
+    def run():
+        ws = torch.empty(n, dtype=torch.uint8, device=C.device) if n else None
+        call("vcsrmc_spmm_mx", dV.handle, *B._args, O, c, ldc, 1 if accumulate else 0, None if ws is None else ws.data_ptr(), n, st)
+
+    _under(guard, run)
     return C
 
 
 def mx_quantize(X, kind: int = MXF8, out: Optional[MXDense] = None, stream=None) -> MXDense:
     """X (float32, float16 or bfloat16) in 8 (MXF8) or 4 bits (MXF4): the scale of 32 columns is the smallest power of two
     under which their largest magnitude fits the element type; elements are rounded to nearest, ties to even."""
-    _dense_2d(X, "X")
-    rows, cols = X.shape
+    x, ldx = _dense_2d(X, "X")
     x_dtype = _dense_dtype(X, "X")
-    with _on(X.device, stream) as on:
-        if out is None:
-            out = MXDense.empty(rows, cols, kind, X.device)
-        elif out.kind != kind or out.shape != (rows, cols) or out.device != X.device:
-            raise _invalid("out must have X's shape and device, and the kind that is asked for")
-        q, q_dtype, ldq, s, lds = out._args()
-        call("vcsrmc_mx_quantize", X.data_ptr(), x_dtype, _row_stride(X), rows, cols, q_dtype, q, ldq, s, lds, on.handle)
-    return out
+    rows, cols = X.shape
+    guard, st = _on(X.device, stream)
+
+    def run():
+        Q = _out_mx(out, rows, cols, kind, X.device)
+        q, q_dtype, ldq, s, lds = Q._args
+        call("vcsrmc_mx_quantize", x, x_dtype, ldx, rows, cols, q_dtype, q, ldq, s, lds, st)
+        return Q
+
+    return _under(guard, run)
 
 
 def mx_dequantize(Q: MXDense, dtype=None, out=None, stream=None):
     """The values an MXDense stands for, rounded to `dtype` (default float32)."""
     import torch
-    with _on(Q.device, stream) as on:
-        if out is None:
-            out = torch.empty(Q.shape, dtype=torch.float32 if dtype is None else dtype, device=Q.device)
-        _dense_2d(out, "out", Q.device, Q.shape, dtype)
-        y_dtype = _dense_dtype(out, "out")
-        call("vcsrmc_mx_dequantize", *Q._args(), Q.rows, Q.cols, out.data_ptr(), y_dtype, _row_stride(out), on.handle)
-    return out
+    guard, st = _on(Q.device, stream)
+
+    def run():
+        Y = torch.empty(Q.rows, Q.cols, dtype=dtype or torch.float32, device=Q.device) if out is None else out
+        y, ldy = _dense_2d(Y, "out", Q.device, Q.shape, dtype)
+        call("vcsrmc_mx_dequantize", *Q._args, Q.rows, Q.cols, y, _dense_dtype(Y, "out"), ldy, st)
+        return Y
+
+    return _under(guard, run)
 
 
 def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, out: Optional[MXDense] = None, residual_out=None,
@@ -513,30 +542,34 @@ def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, 
     eps) of every row (float32); Q = MX(s * inv_rms * weight). The residual has X's type, or X is float32 (a product's C). Without a
     residual s is X, which is then returned in residual_out's place. residual_out may be the residual, or X of the same type (in place)."""
     import torch
-    _dense_2d(X, "X")
-    rows, cols = X.shape
-    x_dtype, w_dtype = _dense_dtype(X, "X"), _dense_dtype(weight, "weight")
-    _vector(weight, "weight", X.device, cols)
-    if residual is not None:
-        _dense_2d(residual, "residual", X.device, X.shape)
-    r_type = X.dtype if residual is None else residual.dtype
-    r_dtype = x_dtype if residual is None else _dense_dtype(residual, "residual")
-    with _on(X.device, stream) as on:
-        if residual_out is not None:
-            _dense_2d(residual_out, "residual_out", X.device, X.shape, r_type)
+    x, ldx = _dense_2d(X, "X")
+    x_dtype, device, shape = _dense_dtype(X, "X"), X.device, X.shape
+    rows, cols = shape
+    w, w_dtype = _vector(weight, "weight", device, cols), _dense_dtype(weight, "weight")
+    if residual is None:
+        r, ldr, r_type, r_dtype = None, 0, X.dtype, x_dtype
+    else:
+        r, ldr = _dense_2d(residual, "residual", device, shape)
+        r_type, r_dtype = residual.dtype, _dense_dtype(residual, "residual")
+    guard, st = _on(device, stream)
+
+    def run():
+        h = residual_out
+        if h is not None:
+            o, ldo = _dense_2d(h, "residual_out", device, shape, r_type)
         elif residual is not None:
-            residual_out = torch.empty((rows, cols), dtype=r_type, device=X.device)
-        if out is None:
-            out = MXDense.empty(rows, cols, kind, X.device)
-        elif out.kind != kind or out.shape != (rows, cols) or out.device != X.device:
-            raise _invalid("out must have X's shape and device, and the kind that is asked for")
-        inv_rms = torch.empty(rows, dtype=torch.float32, device=X.device)
-        q, q_dtype, ldq, s, lds = out._args()
-        call("vcsrmc_add_rms_norm", X.data_ptr(), x_dtype, _row_stride(X),
-             None if residual is None else residual.data_ptr(), 0 if residual is None else _row_stride(residual),
-             None if residual_out is None else residual_out.data_ptr(), 0 if residual_out is None else _row_stride(residual_out), r_dtype,
-             weight.data_ptr(), w_dtype, eps, rows, cols, q_dtype, q, ldq, s, lds, inv_rms.data_ptr(), on.handle)
-    return out, X if residual_out is None else residual_out, inv_rms
+            h = torch.empty(rows, cols, dtype=r_type, device=device)
+            o, ldo = h.data_ptr(), max(cols, 1)
+        else:
+            o, ldo = None, 0
+        Q = _out_mx(out, rows, cols, kind, device)
+        inv_rms = torch.empty(rows, dtype=torch.float32, device=device)
+        q, q_dtype, ldq, s, lds = Q._args
+        call("vcsrmc_add_rms_norm", x, x_dtype, ldx, r, ldr, o, ldo, r_dtype, w, w_dtype, eps, rows, cols, q_dtype, q, ldq, s, lds,
+             inv_rms.data_ptr(), st)
+        return Q, X if h is None else h, inv_rms
+
+    return _under(guard, run)
 
 
 def add_rms_norm_backward(dY, weight, hidden, inv_rms, d_residual=None, out=None, stream=None):
@@ -544,26 +577,35 @@ def add_rms_norm_backward(dY, weight, hidden, inv_rms, d_residual=None, out=None
     counts as the identity), hidden and inv_rms are what the forward call returned, d_residual the gradient of its residual_out. dX, in
     hidden's type, is the gradient of X and of the residual; dweight is float32. out (dX) may be d_residual, or dY of the same type."""
     import torch
-    _dense_2d(dY, "dY")
-    rows, cols = dY.shape
-    dy_dtype, w_dtype = _dense_dtype(dY, "dY"), _dense_dtype(weight, "weight")
-    _vector(weight, "weight", dY.device, cols)
-    _dense_2d(hidden, "hidden", dY.device, dY.shape)
-    _vector(inv_rms, "inv_rms", dY.device, rows, torch.float32)
+    dy, lddy = _dense_2d(dY, "dY")
+    dy_dtype, device, shape = _dense_dtype(dY, "dY"), dY.device, dY.shape
+    rows, cols = shape
+    w, w_dtype = _vector(weight, "weight", device, cols), _dense_dtype(weight, "weight")
+    h, ldh = _dense_2d(hidden, "hidden", device, shape)
     r_dtype = _dense_dtype(hidden, "hidden")
-    if d_residual is not None:
-        _dense_2d(d_residual, "d_residual", dY.device, dY.shape, hidden.dtype)
-    with _on(dY.device, stream) as on:
-        if out is None:
-            out = torch.empty((rows, cols), dtype=hidden.dtype, device=dY.device)
-        _dense_2d(out, "out", dY.device, dY.shape, hidden.dtype)
-        dweight = torch.empty(cols, dtype=torch.float32, device=dY.device)
-        ws, n = _workspace("vcsrmc_add_rms_norm_backward_workspace", dY.device, rows, cols)
-        call("vcsrmc_add_rms_norm_backward", dY.data_ptr(), dy_dtype, _row_stride(dY),
-             None if d_residual is None else d_residual.data_ptr(), 0 if d_residual is None else _row_stride(d_residual),
-             hidden.data_ptr(), _row_stride(hidden), r_dtype, weight.data_ptr(), w_dtype, inv_rms.data_ptr(), rows, cols,
-             out.data_ptr(), _row_stride(out), dweight.data_ptr(), None if ws is None else ws.data_ptr(), n, on.handle)
-    return out, dweight
+    inv = _vector(inv_rms, "inv_rms", device, rows, torch.float32)
+    dr, lddr = (None, 0) if d_residual is None else _dense_2d(d_residual, "d_residual", device, shape, hidden.dtype)
+    guard, st = _on(device, stream)
+
+    def run():
+        dX = torch.empty(rows, cols, dtype=hidden.dtype, device=device) if out is None else out
+        dx, lddx = _dense_2d(dX, "out", device, shape, hidden.dtype)
+        dweight = torch.empty(cols, dtype=torch.float32, device=device)
+        n = _grad_workspace(rows, cols, device.index)
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        call("vcsrmc_add_rms_norm_backward", dy, dy_dtype, lddy, dr, lddr, h, ldh, r_dtype, w, w_dtype, inv, rows, cols, dx, lddx,
+             dweight.data_ptr(), ws.data_ptr(), n, st)
+        return dX, dweight
+
+    return _under(guard, run)
+
+
+@functools.lru_cache(maxsize=256)
+def _grad_workspace(rows: int, cols: int, device: int) -> int:
+    """Bytes of add_rms_norm_backward's workspace; they depend on the shape and the device's SM count."""
+    n = ctypes.c_int64()
+    call("vcsrmc_add_rms_norm_backward_workspace", rows, cols, ctypes.byref(n))
+    return n.value
 
 
 def run_vcsr_mc_spmm_gpu(dV: DeviceVCSRMC, B, O: int, tileK: int, C, stream=None, accumulate: bool = True) -> float:

@@ -581,9 +581,11 @@ RowsLayout build_rows_layout(const int* row_ptr, const int* col, const float* va
     std::vector<RowViewHost::Unit> hunits;
     std::vector<int> hsplit;
     pack_units(hrp.data(), M, unit_nnz, hunits, hsplit);
+    const std::vector<int> hstarts = chunk_starts(hunits);
     static_assert(sizeof(RowViewHost::Unit) == sizeof(int4), "unit layout");
     Buf<int4> units(hunits.size());
-    Buf<int> split(hsplit.size());
+    Buf<int> split(hsplit.size()), starts(hstarts.size());
+    check(cudaMemcpyAsync(starts.p, hstarts.data(), sizeof(int) * hstarts.size(), cudaMemcpyHostToDevice, st), "cudaMemcpyAsync");
     if (!hunits.empty())
         check(cudaMemcpyAsync(units.p, hunits.data(), sizeof(int4) * hunits.size(), cudaMemcpyHostToDevice, st),
               "cudaMemcpyAsync");
@@ -597,7 +599,9 @@ RowsLayout build_rows_layout(const int* row_ptr, const int* col, const float* va
     R.vals = vals.release();
     R.units = units.release();
     R.n_units = n_units;
-    R.n_chunks = count_chunks(hunits);
+    R.chunk_start = starts.release();
+    R.n_chunks = hstarts.back();
+    R.most_chunks = most_chunks(hstarts);
     R.split_rows = split.release();
     R.n_split_rows = int(n_split);
     return R;

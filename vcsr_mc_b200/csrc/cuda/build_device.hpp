@@ -28,7 +28,9 @@ struct RowsLayout {
     void* vals = nullptr;  // __half (FP16 format) or float
     int4* units = nullptr;
     int64_t n_units = 0, n_chunks = 0;
+    int most_chunks = 0;
     int* split_rows = nullptr;
+    int* chunk_start = nullptr;
     int n_split_rows = 0;
 };
 

@@ -53,6 +53,8 @@ struct vcsrmc_device_format {
     int* cols = nullptr;
     void* rvals = nullptr;
     int* split_rows = nullptr;
+    int* chunk_start = nullptr;
+    int most_chunks = 0;
     int n_split_rows = 0;
     int unit_nnz = 0;
     // BAND plan
@@ -146,6 +148,7 @@ void free_device(vcsrmc_device_format* d) {
     cudaFree(d->cols);
     cudaFree(d->rvals);
     cudaFree(d->split_rows);
+    cudaFree(d->chunk_start);
     cudaFree(d->tile_ptr);
     cudaFree(d->tile_col);
     cudaFree(d->tile_eptr);
@@ -570,7 +573,10 @@ VCSRMC_EXPORT int vcsrmc_upload_opts(const vcsrmc_format* f, int device, const v
                 static_assert(sizeof(dev::RowViewHost::Unit) == sizeof(int4), "unit layout");
                 d->units = reinterpret_cast<int4*>(upload_array(rv.units.data(), rv.units.size(), st));
                 d->n_units = int64_t(rv.units.size());
-                d->n_chunks = dev::count_chunks(rv.units);
+                const std::vector<int> starts = dev::chunk_starts(rv.units);
+                d->chunk_start = upload_array(starts.data(), starts.size(), st);
+                d->n_chunks = starts.back();
+                d->most_chunks = dev::most_chunks(starts);
                 d->split_rows = upload_array(rv.split_rows.data(), rv.split_rows.size(), st);
                 d->n_split_rows = int(rv.split_rows.size());
                 d->unit_nnz = unit_nnz;
@@ -811,7 +817,9 @@ VCSRMC_EXPORT int vcsrmc_build_device(int32_t M, int32_t N, int64_t nnz, const i
                 d->rvals = rows.vals;
                 d->units = rows.units;
                 d->n_units = rows.n_units;
+                d->chunk_start = rows.chunk_start;
                 d->n_chunks = rows.n_chunks;
+                d->most_chunks = rows.most_chunks;
                 d->split_rows = rows.split_rows;
                 d->n_split_rows = rows.n_split_rows;
                 d->unit_nnz = unit_nnz;
@@ -1010,7 +1018,31 @@ int sm_count() {
     return sms;
 }
 
-int64_t spmm_mx_bytes(const vcsrmc_device_format* d, int32_t O) { return d->n_chunks * int64_t(O) * int64_t(sizeof(float)); }
+// The ROWS layout as a product with an MX operand reads it.
+dev::RowPlanView mx_plan(const vcsrmc_device_format* d) {
+    dev::RowPlanView P;
+    P.units = d->units;
+    P.n_units = d->n_units;
+    P.rp = d->rp;
+    P.cols = d->cols;
+    P.vals = d->rvals;
+    P.vals_f16 = d->fp32 ? 0 : 1;
+    P.split_rows = d->split_rows;
+    P.n_split_rows = d->n_split_rows;
+    P.chunk_start = d->chunk_start;
+    P.n_chunks = d->n_chunks;
+    P.most_chunks = d->most_chunks;
+    P.unit_nnz = d->unit_nnz;
+    P.M = d->M;
+    P.N = d->N;
+    P.scale = d->scale;
+    P.hot.hot_cols = d->hot_cols;
+    return P;
+}
+
+int64_t spmm_mx_bytes(const vcsrmc_device_format* d, int32_t O) {
+    return dev::rows_mx_chunks(mx_plan(d)) * dev::rows_mx_pitch(O) * int64_t(sizeof(float));
+}
 
 void check_spmm_mx(const vcsrmc_device_format* d, int32_t O) {
     if (!d) invalid("NULL format");
@@ -1061,21 +1093,7 @@ VCSRMC_EXPORT int vcsrmc_spmm_mx(const vcsrmc_device_format* d, const void* Q, i
             invalid("the workspace is smaller than vcsrmc_spmm_mx_workspace says: " + std::to_string(need) + " bytes");
         if (reinterpret_cast<uintptr_t>(workspace) % 16) invalid("the workspace must be 16-byte aligned");
         DeviceGuard guard(d->device);
-        dev::RowPlanView P;
-        P.units = d->units;
-        P.n_units = d->n_units;
-        P.rp = d->rp;
-        P.cols = d->cols;
-        P.vals = d->rvals;
-        P.vals_f16 = d->fp32 ? 0 : 1;
-        P.split_rows = d->split_rows;
-        P.n_split_rows = d->n_split_rows;
-        P.n_chunks = d->n_chunks;
-        P.M = d->M;
-        P.N = d->N;
-        P.scale = d->scale;
-        P.hot.hot_cols = d->hot_cols;
-        cuda_check(dev::spmm_rows_mx(P, q, O, static_cast<float*>(c.p), ldc, accumulate != 0, static_cast<float*>(workspace),
+        cuda_check(dev::spmm_rows_mx(mx_plan(d), q, O, static_cast<float*>(c.p), ldc, accumulate != 0, static_cast<float*>(workspace),
                                      static_cast<cudaStream_t>(stream)),
                    "SpMM launch (rows plan, microscaled B)");
     });

@@ -59,6 +59,10 @@ __device__ __forceinline__ float2 mx_f16x2_to_f32(uint32_t h) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// ---- a launch that starts while the one before it in the stream ends ----------------------------
+// The host side's attribute lets it start, and its blocks wait here for the other's results.
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- dense elements (fp32, fp16, bf16) ---------------------------------------------------------
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -160,6 +164,22 @@ __device__ __forceinline__ void mx_store_block(const float (&y)[8], int nv, bool
                 if (i < nv) q[i] = uint8_t(w[i >> 2] >> (8 * (i & 3)));
         }
     }
+}
+
+// The same for a block held one column per lane by a warp: q is the column's place in the row; `next`:
+// the next column exists too (two E2M1 elements share a byte, which the even column writes).
+__device__ __forceinline__ void mx_store_column(float y, bool exists, bool next, bool q4, uint8_t* q, uint8_t* s) {
+    const uint32_t amax = __reduce_max_sync(0xffffffffu, exists ? __float_as_uint(y) & 0x7fffffffu : 0u);
+    const uint32_t code = mx_scale_code(amax, q4);
+    const float t = code == kMxNan || !exists ? 0.f : y * mx_inverse_scale(code);
+    const int lane = threadIdx.x & 31;
+    if (q4) {
+        const float u = __shfl_down_sync(0xffffffffu, t, 1);
+        if (exists && !(lane & 1)) *q = uint8_t(mx_encode2_e2m1(t, next ? u : 0.f));
+    } else {
+        if (exists) *q = uint8_t(mx_encode2_e4m3(t, 0.f));
+    }
+    if (exists && lane == 0) *s = uint8_t(code);
 }
 
 }  // namespace dev

@@ -10,6 +10,22 @@
 namespace vcsrmc {
 namespace dev {
 
+// Configuration of a launch whose blocks may start before the launch ahead of them in the stream has ended (they
+// wait for it themselves, wait_for_launch_before in mx.cuh).
+struct LaunchAfter {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    LaunchAfter(dim3 grid, dim3 block, cudaStream_t st) {
+        cfg.gridDim = grid;
+        cfg.blockDim = block;
+        cfg.stream = st;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+    }
+};
+
 // A strided row-major matrix of fp32, fp16 or bf16 (VCSRMC_F32, _F16, _BF16); ld in elements.
 struct DenseView {
     void* p = nullptr;
@@ -35,6 +51,7 @@ struct RmsNormArgs {
     DenseView x, residual, residual_out;
     const void* weight = nullptr;
     int w_dtype = 0;
+    bool vec_w = false;  // the weight is 16-byte aligned (set by the launcher)
     float eps = 0.f;
     int64_t rows = 0;
     int O = 0;
@@ -47,6 +64,7 @@ struct RmsNormGradArgs {
     DenseView dy, d_residual, hidden, dx;
     const void* weight = nullptr;
     int w_dtype = 0;
+    bool vec_w = false;  // the weight is 16-byte aligned (set by the launcher)
     const float* inv_rms = nullptr;
     int64_t rows = 0;
     int O = 0;
@@ -56,8 +74,11 @@ struct RmsNormGradArgs {
 int64_t rms_norm_grad_workspace(int64_t rows, int O, int sms);
 cudaError_t add_rms_norm_backward(const RmsNormGradArgs& a, int sms, cudaStream_t st);
 
-// C (+)= A * B with an MX operand B over the row view. `partial`: P.n_chunks * O floats (null when
-// P.n_chunks is 0), one row for every chunk of a split row; they are summed in chunk order.
+// C (+)= A * B with an MX operand B over the row view. `partial`: rows_mx_chunks(P) rows of rows_mx_pitch(O)
+// floats, 16-byte aligned (null when there are none), one for every chunk of a split row; they are summed in
+// chunk order.
+int64_t rows_mx_chunks(const RowPlanView& P);
+int64_t rows_mx_pitch(int O);
 cudaError_t spmm_rows_mx(const RowPlanView& P, const MxView& B, int O, float* C, int64_t ldc, bool accumulate,
                          float* partial, cudaStream_t st);
 

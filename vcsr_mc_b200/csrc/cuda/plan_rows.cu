@@ -681,9 +681,19 @@ void pack_units(const int* rp, int M, int unit_nnz, std::vector<RowViewHost::Uni
     }
 }
 
-int64_t count_chunks(const std::vector<RowViewHost::Unit>& units) {
-    const auto light = std::find_if(units.begin(), units.end(), [](const RowViewHost::Unit& u) { return u.y >= 0; });
-    return int64_t(light - units.begin());
+std::vector<int> chunk_starts(const std::vector<RowViewHost::Unit>& units) {
+    std::vector<int> starts;
+    size_t i = 0;
+    for (; i < units.size() && units[i].y < 0; ++i)
+        if (i == 0 || units[i].x != units[i - 1].x) starts.push_back(int(i));
+    starts.push_back(int(i));
+    return starts;
+}
+
+int most_chunks(const std::vector<int>& starts) {
+    int most = 0;
+    for (size_t i = 1; i < starts.size(); ++i) most = std::max(most, starts[i] - starts[i - 1]);
+    return most;
 }
 
 RowViewHost build_row_view(const VCSRMC& v, int unit_nnz) {

@@ -32,8 +32,11 @@ RowViewHost build_row_view(const VCSRMC& v, int unit_nnz);
 // store; a run may still hold empty rows between non-empty ones).
 void pack_units(const int* rp, int M, int unit_nnz, std::vector<RowViewHost::Unit>& units,
                 std::vector<int>& split_rows, bool skip_empty = false);
-// Units that are chunks of split rows: they come first, in the order of their rows.
-int64_t count_chunks(const std::vector<RowViewHost::Unit>& units);
+// First unit of each split row's chunks, and the unit after the last of them: chunks come first among the
+// units, in the order of their rows.
+std::vector<int> chunk_starts(const std::vector<RowViewHost::Unit>& units);
+// The largest number of chunks of one row, from chunk_starts.
+int most_chunks(const std::vector<int>& starts);
 // The unit size for a matrix of `nnz` entries on a GPU with `sms` SMs: the largest power of two
 // in [16, 256] that still gives every resident lane group (48 per SM) about four units.
 int choose_unit_nnz(int64_t nnz, int sms);
@@ -63,7 +66,10 @@ struct RowPlanView {
     int vals_f16;
     const int* split_rows;
     int n_split_rows;
-    int64_t n_chunks = 0;  // leading units that are chunks of split rows
+    const int* chunk_start = nullptr;  // n_split_rows + 1: first chunk of each split row
+    int64_t n_chunks = 0;              // leading units that are chunks of split rows
+    int most_chunks = 0;               // of one row
+    int unit_nnz = 0;                  // entries per chunk
     int M;
     int N = 0;  // columns of A (rows of B): bounds the B row offsets the kernel forms
     float scale;

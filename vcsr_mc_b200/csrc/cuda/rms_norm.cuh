@@ -1,0 +1,402 @@
+// Residual addition with root-mean-square norm, written as a microscaled (MX) matrix, and its
+// backward pass. For a row of O columns:
+//   s = round(x + residual)              (to the residual's type; the next residual)
+//   inv = 1 / sqrt(mean(s^2) + eps)
+//   Q = MX(s * inv * w)                  (mx.cuh)
+// and with dy the gradient of the values that Q stands for (the element's rounding counts as identity),
+// n = s * inv and g = dy * w:
+//   dx = d_residual + inv * (g - n * mean(g * n))
+//   dw = sum over rows of dy * n
+// The square sums are held in 64 bits: fp32 would overflow for |s| above 2^64, which bf16 and fp32 can
+// hold; the backward pass sums products of the normalised n, which cannot. Both passes read each input
+// once and write each output once (a row stays in registers up to 16384 columns forward and 8192 backward,
+// and is read a second time beyond), so HBM bounds them except for a few rows.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "mx.cuh"
+#include "mx.hpp"
+#include "vcsrmc.h"
+
+namespace vcsrmc {
+namespace dev {
+namespace norm {
+
+// How a row lies over threads. kV = 8: a thread holds groups of eight consecutive columns (16-byte loads and
+// stores; O is a multiple of 8 and every row aligned), kV = 1: single columns, neighbouring threads
+// neighbouring columns, for every other layout. kN columns per thread in all, on kL lanes of a warp or, for
+// kL = 0, on the whole block. kN = 0: any width in steps of 8, the row is read twice.
+template <int kV_, int kL_, int kN_, int kThreads_ = 256>
+struct Span {
+    static constexpr int kV = kV_, kL = kL_;
+    static constexpr bool kAny = kN_ == 0;
+    static constexpr int kN = kAny ? 8 : kN_;  // columns held at once
+    static constexpr int kThreads = kThreads_;     // per block, at most
+    static constexpr int kRows = kL_ ? 256 / (kL_ ? kL_ : 1) : 1;  // rows in a block
+    static_assert(kN % kV == 0 && (kV == 8 || kL == 0 || kL == 32), "whole groups; single columns on whole warps");
+    __device__ static int per_row() { return kL ? kL : int(blockDim.x); }
+    __device__ static int slot() { return kL ? int(threadIdx.x) % (kL ? kL : 1) : int(threadIdx.x); }
+    __device__ static int row_in_block() { return kL ? int(threadIdx.x) / (kL ? kL : 1) : 0; }
+    // column of this thread's element i, `step` kN-wide steps into the row
+    __device__ static int column(int i, int step = 0) {
+        const int at = step * (kN / kV) + i / kV;
+        return kV * (at * per_row() + slot()) + i % kV;
+    }
+};
+
+// A thread's columns as they were read; converted when they are used, so that all loads are in flight first.
+// kWide: fp32, else fp16 or bf16 (two to a word where a thread holds groups of eight).
+template <class S, bool kWide>
+struct Held {
+    static constexpr int kPer = S::kV == 8 && !kWide ? 2 : 1;  // elements per word
+    uint32_t w[S::kN / kPer];
+};
+
+template <class S, bool kWide>
+__device__ __forceinline__ void load(Held<S, kWide>& r, const DenseView& v, int64_t row, int O, int step = 0) {
+    using T = typename std::conditional<kWide, uint32_t, unsigned short>::type;
+    const T* p = static_cast<const T*>(v.p) + row * v.ld;
+#pragma unroll
+    for (int i = 0; i < S::kN; i += S::kV) {
+        const int c = S::column(i, step);
+        if constexpr (S::kV == 8) {
+#pragma unroll
+            for (int k = 0; k < (kWide ? 2 : 1); ++k) {
+                const uint4 a = c < O ? __ldcs(reinterpret_cast<const uint4*>(p + c) + k) : make_uint4(0, 0, 0, 0);
+                uint32_t* w = r.w + i / Held<S, kWide>::kPer + 4 * k;
+                w[0] = a.x;
+                w[1] = a.y;
+                w[2] = a.z;
+                w[3] = a.w;
+            }
+        } else {
+            r.w[i] = c < O ? p[c] : 0u;
+        }
+    }
+}
+
+// Calls fn with the element type of a dense dtype (kWide says which are possible). The type is uniform, so this
+// is one branch around the loops of a row and not one in them.
+template <bool kWide, class Fn>
+__device__ __forceinline__ void with_type(int dtype, Fn&& fn) {
+    if constexpr (kWide) fn(float{});
+    else if (dtype == VCSRMC_F16) fn(__half{});
+    else fn(__nv_bfloat16{});
+}
+
+template <class S, bool kWide>
+__device__ __forceinline__ void to_floats(const Held<S, kWide>& r, int dtype, float (&v)[S::kN]) {
+    with_type<kWide>(dtype, [&](auto t) {
+        using T = decltype(t);
+#pragma unroll
+        for (int i = 0; i < S::kN; ++i) v[i] = to_f32(reinterpret_cast<const T*>(&r.w[i / Held<S, kWide>::kPer])[i % Held<S, kWide>::kPer]);
+    });
+}
+
+template <class S, bool kWide>
+__device__ __forceinline__ void store(const float (&v)[S::kN], const DenseView& d, int64_t row, int O, int step = 0) {
+    with_type<kWide>(d.dtype, [&](auto t) {
+        using T = decltype(t);
+        T* p = static_cast<T*>(d.p) + row * d.ld;
+#pragma unroll
+        for (int i = 0; i < S::kN; i += S::kV) {
+            const int c = S::column(i, step);
+            if (c >= O) continue;
+            if constexpr (S::kV == 8) {
+                float u[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) u[k] = v[i + k];
+                store8(p + c, 8, true, u);
+            } else {
+                p[c] = from_f32<T>(v[i]);
+            }
+        }
+    });
+}
+
+// The weights of a thread's columns (0 past the row's end).
+template <class S>
+__device__ __forceinline__ void load_weights(float (&w)[S::kN], const void* weight, int dtype, bool vec, int O, int step = 0) {
+    auto read = [&](auto t) {
+        using T = decltype(t);
+        const T* p = static_cast<const T*>(weight);
+#pragma unroll
+        for (int i = 0; i < S::kN; i += S::kV) {
+            const int c = S::column(i, step);
+            if constexpr (S::kV == 8) {
+                float u[8];
+                load8(p + c, c < O ? 8 : 0, vec, u);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[i + k] = u[k];
+            } else {
+                w[i] = c < O ? to_f32(p[c]) : 0.f;
+            }
+        }
+    };
+    if (dtype == VCSRMC_F32) read(float{});
+    else with_type<false>(dtype, read);
+}
+
+// Sum over the lanes of a row, or over the block (kL = 0); every thread gets the result. The order of the
+// additions depends on the thread count alone.
+template <class S, typename T>
+__device__ __forceinline__ T row_sum(T v, T* smem) {
+    constexpr int kW = S::kL == 0 ? 32 : S::kL;
+#pragma unroll
+    for (int d = kW / 2; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if constexpr (S::kL == 0) {
+        const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+        __syncthreads();  // smem may still be read from the row before
+        if (lane == 0) smem[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = lane < warps ? smem[lane] : T(0);
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    }
+    return v;
+}
+
+// 1 / sqrt(v), rounded once to fp32: the hardware's estimate and a Newton step in 64 bits (its error squared,
+// below 2^-40), or 64-bit operations where v leaves the estimate's range.
+__device__ __forceinline__ float inverse_root(double v) {
+    if (v > 1e-30 && v < 1e30) {
+        const double r = double(rsqrtf(float(v)));
+        return float(r * (1.5 - 0.5 * v * r * r));
+    }
+    return float(1.0 / sqrt(v));
+}
+
+template <class S, bool kXWide, bool kRWide>
+__global__ void __launch_bounds__(S::kThreads) rms_norm_kernel(RmsNormArgs a) {
+    __shared__ double smem[32];
+    const int64_t row = int64_t(blockIdx.x) * S::kRows + S::row_in_block();
+    const bool live = row < a.rows;  // every thread takes part in the reductions of a row past the end
+    const int O = live ? a.O : 0;
+    const int r_dtype = a.residual_out.dtype;
+    const int steps = S::kAny ? (a.O + S::kN * S::per_row() - 1) / (S::kN * S::per_row()) : 1;
+    float s[S::kN];
+    auto load_sum = [&](int step) {
+        Held<S, kXWide> x;
+        Held<S, kRWide> r;
+        load(x, a.x, row, O, step);
+        if (a.residual.p) {
+            load(r, a.residual, row, O, step);
+            float t[S::kN];
+            to_floats(x, a.x.dtype, s);
+            to_floats(r, r_dtype, t);
+#pragma unroll
+            for (int i = 0; i < S::kN; ++i) s[i] += t[i];
+        } else {
+            to_floats(x, a.x.dtype, s);
+        }
+        with_type<kRWide>(r_dtype, [&](auto t) {
+#pragma unroll
+            for (int i = 0; i < S::kN; ++i) s[i] = to_f32(from_f32<decltype(t)>(s[i]));
+        });
+    };
+    double sum = 0.0;
+    for (int k = 0; k < steps; ++k) {
+        load_sum(k);
+#pragma unroll
+        for (int i = 0; i < S::kN; ++i) sum = fma(double(s[i]), double(s[i]), sum);
+    }
+    sum = row_sum<S>(sum, smem);
+    const float inv = inverse_root(sum / double(a.O) + double(a.eps));
+    if (live && S::slot() == 0 && a.inv_rms) a.inv_rms[row] = inv;
+    uint8_t* q = a.out.q + row * a.out.ldq;
+    uint8_t* scales = a.out.s + row * a.out.lds;
+    for (int k = 0; k < steps; ++k) {
+        if constexpr (S::kAny) load_sum(k);
+        if (a.residual_out.p) store<S, kRWide>(s, a.residual_out, row, O, k);
+        float w[S::kN];
+        load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, O, k);
+#pragma unroll
+        for (int i = 0; i < S::kN; i += S::kV) {
+            const int c = S::column(i, k);
+            if constexpr (S::kV == 8) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = s[i + j] * inv * w[i + j];
+                mx_store_block(y, c < O ? 8 : 0, a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock, true);
+            } else {
+                const float y = s[i] * inv * w[i];
+                mx_store_column(y, c < O, c + 1 < O, a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock);
+            }
+        }
+    }
+}
+
+// ---- backward --------------------------------------------------------------------------------------
+// Persistent blocks over the rows; each thread keeps the weight gradient of its columns in registers
+// and the block writes one row of partial sums to the workspace, in which a second kernel adds the
+// blocks up in their order. Registers are held to 64 a thread: the pass waits for memory, and 1024 threads per SM
+// hide it better than 512 with more registers (rows of 128: 233 against 265 us, of 4096: 234 against 347 us).
+template <class S, bool kYWide, bool kRWide>
+__global__ void __launch_bounds__(S::kThreads, S::kL ? 4 : 2) rms_norm_grad_kernel(RmsNormGradArgs a) {
+    __shared__ float smem[32];
+    __shared__ float fold[S::kL ? 8 : 1][S::kL ? 257 : 1];
+    const int steps = S::kAny ? (a.O + S::kN * S::per_row() - 1) / (S::kN * S::per_row()) : 1;
+    float* part = a.workspace + int64_t(blockIdx.x) * a.O;
+    float dw[S::kN] = {}, w[S::kN];
+    if constexpr (!S::kAny) load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, a.O);
+    for (int64_t r0 = int64_t(blockIdx.x) * S::kRows; r0 < a.rows; r0 += int64_t(gridDim.x) * S::kRows) {
+        const int64_t row = r0 + S::row_in_block();
+        const bool live = row < a.rows;
+        const int O = live ? a.O : 0;
+        Held<S, kYWide> dy;
+        Held<S, kRWide> h, dr;
+        const float inv = live ? a.inv_rms[row] : 0.f;
+        auto load_step = [&](int k) {
+            load(dy, a.dy, row, O, k);
+            load(h, a.hidden, row, O, k);
+            if constexpr (S::kAny) load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, O, k);
+        };
+        // the gradient g = dy * w is 0 past the row's end, where w is, and so are its products
+        float dot = 0.f;
+        for (int k = 0; k < steps; ++k) {
+            load_step(k);
+            if (!S::kAny && a.d_residual.p) load(dr, a.d_residual, row, O);
+            float vy[S::kN], vh[S::kN];
+            to_floats(dy, a.dy.dtype, vy);
+            to_floats(h, a.hidden.dtype, vh);
+#pragma unroll
+            for (int i = 0; i < S::kN; ++i) dot = fmaf(vy[i] * w[i], vh[i] * inv, dot);
+        }
+        const float m = row_sum<S>(dot, smem) / float(a.O);
+        for (int k = 0; k < steps; ++k) {
+            if constexpr (S::kAny) {
+                load_step(k);
+                if (a.d_residual.p) load(dr, a.d_residual, row, O, k);
+            }
+            float vy[S::kN], vh[S::kN], dx[S::kN] = {};
+            to_floats(dy, a.dy.dtype, vy);
+            to_floats(h, a.hidden.dtype, vh);
+            if (a.d_residual.p) to_floats(dr, a.hidden.dtype, dx);
+#pragma unroll
+            for (int i = 0; i < S::kN; ++i) {
+                const float n = vh[i] * inv;
+                dx[i] = fmaf(inv, fmaf(vy[i], w[i], -(n * m)), dx[i]);
+                if constexpr (S::kAny) {
+                    const int c = S::column(i, k);
+                    if (c < O) part[c] = fmaf(vy[i], n, r0 == int64_t(blockIdx.x) ? 0.f : part[c]);
+                } else {
+                    dw[i] = fmaf(vy[i], n, dw[i]);
+                }
+            }
+            store<S, kRWide>(dx, a.dx, row, O, k);
+        }
+    }
+    if constexpr (!S::kAny && S::kL > 0) {
+        // sum over the rows of the block, in their order, eight elements of every thread at a time
+#pragma unroll
+        for (int i0 = 0; i0 < S::kN; i0 += 8) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8 && i0 + i < S::kN; ++i) fold[i][threadIdx.x] = dw[i0 + i];
+            __syncthreads();
+            for (int t = int(threadIdx.x); t < S::kL * 8; t += 256) {
+                const int i = t / S::kL, slot = t % S::kL;
+                const int at = (i0 + i) / S::kV;
+                const int c = S::kV * (at * S::kL + slot) + (i0 + i) % S::kV;
+                if (i0 + i < S::kN && c < a.O) {
+                    float v = 0.f;
+                    for (int g = 0; g < S::kRows; ++g) v += fold[i][g * S::kL + slot];
+                    part[c] = v;
+                }
+            }
+        }
+    } else if constexpr (!S::kAny) {
+#pragma unroll
+        for (int i = 0; i < S::kN; ++i)
+            if (S::column(i) < a.O) part[S::column(i)] = dw[i];
+    }
+}
+
+inline bool aligned(const void* p, int64_t ld_bytes, int64_t to) {
+    return reinterpret_cast<uintptr_t>(p) % uintptr_t(to) == 0 && ld_bytes % to == 0;
+}
+inline bool aligned16(const DenseView& v) { return aligned(v.p, v.ld * (v.dtype == VCSRMC_F32 ? 4 : 2), 16); }
+
+// Threads that hold O columns, n each, in whole warps.
+inline int threads_for(int O, int n) { return ((O + n - 1) / n + 31) / 32 * 32; }
+// Threads of a backward block that holds one row (O > 256): 8 columns each up to 4096 columns, 16 up to 8192.
+inline int grad_threads(int O) { return std::min(512, threads_for(O, O <= 4096 ? 8 : 16)); }
+
+template <class S, bool kXWide, bool kRWide>
+cudaError_t launch_norm(const RmsNormArgs& a, int threads, cudaStream_t st) {
+    const int64_t blocks = (a.rows + S::kRows - 1) / S::kRows;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    rms_norm_kernel<S, kXWide, kRWide><<<unsigned(blocks), S::kL ? 256 : threads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <class S, bool kYWide, bool kRWide>
+cudaError_t launch_grad(const RmsNormGradArgs& a, int threads, int64_t blocks, cudaStream_t st) {
+    rms_norm_grad_kernel<S, kYWide, kRWide><<<unsigned(blocks), S::kL ? 256 : threads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+// The launches of one pair of element widths (X or dY, residual); each pair is a translation unit.
+template <bool kXWide, bool kRWide>
+cudaError_t forward(const RmsNormArgs& a, cudaStream_t st) {
+    const int O = a.O;
+    const bool vec = O % 8 == 0 && aligned16(a.x) && (!a.residual.p || aligned16(a.residual)) &&
+                     (!a.residual_out.p || aligned16(a.residual_out)) && aligned(a.out.q, a.out.ldq, a.out.q4 ? 4 : 8);
+    if (vec) {
+        if (O <= 32) return launch_norm<Span<8, 4, 8>, kXWide, kRWide>(a, 0, st);
+        if (O <= 64) return launch_norm<Span<8, 8, 8>, kXWide, kRWide>(a, 0, st);
+        if (O <= 128) return launch_norm<Span<8, 16, 8>, kXWide, kRWide>(a, 0, st);
+        if (O <= 256) return launch_norm<Span<8, 32, 8>, kXWide, kRWide>(a, 0, st);
+        if (O <= 512) return launch_norm<Span<8, 32, 16>, kXWide, kRWide>(a, 0, st);
+        if (O <= 1024) return launch_norm<Span<8, 32, 32>, kXWide, kRWide>(a, 0, st);
+        if (O <= 8 * 1024) return launch_norm<Span<8, 0, 8, 1024>, kXWide, kRWide>(a, threads_for(O, 8), st);
+        if (O <= 16 * 1024) return launch_norm<Span<8, 0, 16, 1024>, kXWide, kRWide>(a, threads_for(O, 16), st);
+        return launch_norm<Span<8, 0, 0, 1024>, kXWide, kRWide>(a, 1024, st);
+    }
+    if (O <= 32) return launch_norm<Span<1, 32, 1>, kXWide, kRWide>(a, 0, st);
+    if (O <= 64) return launch_norm<Span<1, 32, 2>, kXWide, kRWide>(a, 0, st);
+    if (O <= 128) return launch_norm<Span<1, 32, 4>, kXWide, kRWide>(a, 0, st);
+    if (O <= 256) return launch_norm<Span<1, 32, 8>, kXWide, kRWide>(a, 0, st);
+    if (O <= 512) return launch_norm<Span<1, 32, 16>, kXWide, kRWide>(a, 0, st);
+    if (O <= 1024) return launch_norm<Span<1, 32, 32>, kXWide, kRWide>(a, 0, st);
+    if (O <= 8 * 1024) return launch_norm<Span<1, 0, 8, 1024>, kXWide, kRWide>(a, threads_for(O, 8), st);
+    if (O <= 16 * 1024) return launch_norm<Span<1, 0, 16, 1024>, kXWide, kRWide>(a, threads_for(O, 16), st);
+    return launch_norm<Span<1, 0, 0, 1024>, kXWide, kRWide>(a, 1024, st);
+}
+
+template <bool kYWide, bool kRWide>
+cudaError_t backward(const RmsNormGradArgs& a, int64_t blocks, cudaStream_t st) {
+    const int O = a.O;
+    const bool vec = O % 8 == 0 && aligned16(a.dy) && aligned16(a.hidden) && aligned16(a.dx) && (!a.d_residual.p || aligned16(a.d_residual));
+    const int threads = grad_threads(O);
+    if (vec) {
+        if (O <= 32) return launch_grad<Span<8, 4, 8>, kYWide, kRWide>(a, 0, blocks, st);
+        if (O <= 64) return launch_grad<Span<8, 8, 8>, kYWide, kRWide>(a, 0, blocks, st);
+        if (O <= 128) return launch_grad<Span<8, 16, 8>, kYWide, kRWide>(a, 0, blocks, st);
+        if (O <= 256) return launch_grad<Span<8, 32, 8>, kYWide, kRWide>(a, 0, blocks, st);
+        if (O <= 4096) return launch_grad<Span<8, 0, 8, 512>, kYWide, kRWide>(a, threads, blocks, st);
+        if (O <= 8192) return launch_grad<Span<8, 0, 16, 512>, kYWide, kRWide>(a, threads, blocks, st);
+        return launch_grad<Span<8, 0, 0, 512>, kYWide, kRWide>(a, threads, blocks, st);
+    }
+    if (O <= 32) return launch_grad<Span<1, 32, 1>, kYWide, kRWide>(a, 0, blocks, st);
+    if (O <= 64) return launch_grad<Span<1, 32, 2>, kYWide, kRWide>(a, 0, blocks, st);
+    if (O <= 128) return launch_grad<Span<1, 32, 4>, kYWide, kRWide>(a, 0, blocks, st);
+    if (O <= 256) return launch_grad<Span<1, 32, 8>, kYWide, kRWide>(a, 0, blocks, st);
+    if (O <= 4096) return launch_grad<Span<1, 0, 8, 512>, kYWide, kRWide>(a, threads, blocks, st);
+    if (O <= 8192) return launch_grad<Span<1, 0, 16, 512>, kYWide, kRWide>(a, threads, blocks, st);
+    return launch_grad<Span<1, 0, 0, 512>, kYWide, kRWide>(a, threads, blocks, st);
+}
+
+extern template cudaError_t forward<true, true>(const RmsNormArgs&, cudaStream_t);
+extern template cudaError_t forward<true, false>(const RmsNormArgs&, cudaStream_t);
+extern template cudaError_t forward<false, false>(const RmsNormArgs&, cudaStream_t);
+extern template cudaError_t backward<true, true>(const RmsNormGradArgs&, int64_t, cudaStream_t);
+extern template cudaError_t backward<true, false>(const RmsNormGradArgs&, int64_t, cudaStream_t);
+extern template cudaError_t backward<false, false>(const RmsNormGradArgs&, int64_t, cudaStream_t);
+
+}  // namespace norm
+}  // namespace dev
+}  // namespace vcsrmc
