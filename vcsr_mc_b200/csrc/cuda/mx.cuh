@@ -17,13 +17,12 @@ namespace dev {
 constexpr int kMxBlock = 32;       // columns per scale
 constexpr uint32_t kMxNan = 255u;  // scale code of a block with an infinity or a NaN
 
-// Scale code of a block from the bits of its largest |x| (a NaN's bits are above infinity's).
+// Scale code of a block from the bits of its largest |x| (a NaN's bits are above infinity's): the exponent, one
+// more where the mantissa is above the element type's largest (the sum carries into the exponent), less the
+// exponent of that largest. A subnormal clamps to code 0.
 __device__ __forceinline__ uint32_t mx_scale_code(uint32_t amax_bits, bool q4) {
-    if (amax_bits >= 0x7f800000u) return kMxNan;
-    const int k = int(amax_bits >> 23);  // amax = 1.m * 2^(k - 127); a subnormal (k = 0) clamps to code 0
-    const uint32_t m = amax_bits & 0x7fffffu;
-    const int code = q4 ? k - 2 + (m > 0x400000u) : k - 8 + (m > 0x600000u);
-    return uint32_t(max(code, 0));
+    const int code = int((amax_bits + (q4 ? 0x3fffffu : 0x1fffffu)) >> 23) - (q4 ? 2 : 8);
+    return amax_bits >= 0x7f800000u ? kMxNan : uint32_t(max(code, 0));
 }
 // 2^-e of a finite block's code (codes reach 253 at most, so this is a normal number).
 __device__ __forceinline__ float mx_inverse_scale(uint32_t code) { return __uint_as_float((254u - code) << 23); }
@@ -166,20 +165,27 @@ __device__ __forceinline__ void mx_store_block(const float (&y)[8], int nv, bool
     }
 }
 
-// The same for a block held one column per lane by a warp: q is the column's place in the row; `next`:
-// the next column exists too (two E2M1 elements share a byte, which the even column writes).
-__device__ __forceinline__ void mx_store_column(float y, bool exists, bool next, bool q4, uint8_t* q, uint8_t* s) {
-    const uint32_t amax = __reduce_max_sync(0xffffffffu, exists ? __float_as_uint(y) & 0x7fffffffu : 0u);
-    const uint32_t code = mx_scale_code(amax, q4);
-    const float t = code == kMxNan || !exists ? 0.f : y * mx_inverse_scale(code);
-    const int lane = threadIdx.x & 31;
-    if (q4) {
-        const float u = __shfl_down_sync(0xffffffffu, t, 1);
-        if (exists && !(lane & 1)) *q = uint8_t(mx_encode2_e2m1(t, next ? u : 0.f));
-    } else {
-        if (exists) *q = uint8_t(mx_encode2_e4m3(t, 0.f));
-    }
-    if (exists && lane == 0) *s = uint8_t(code);
+// From columns dealt out over kL neighbouring lanes (t[j] is column j * kL + lane of a span of 8 * kL, as coalesced
+// single loads give them) to eight consecutive columns per lane, or back. `span`: 8 * kL floats of shared memory
+// that are the lanes' own, 16-byte aligned. All lanes of the warp take part.
+template <int kL>
+__device__ __forceinline__ void turn_to_groups(const float (&t)[8], float (&v)[8], float* span, int sl) {
+    __syncwarp();  // the span may still be read
+#pragma unroll
+    for (int j = 0; j < 8; ++j) span[j * kL + sl] = t[j];
+    __syncwarp();
+    const float4 a = *reinterpret_cast<const float4*>(span + 8 * sl), b = *reinterpret_cast<const float4*>(span + 8 * sl + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <int kL>
+__device__ __forceinline__ void turn_to_columns(const float (&v)[8], float (&t)[8], float* span, int sl) {
+    __syncwarp();
+    *reinterpret_cast<float4*>(span + 8 * sl) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(span + 8 * sl + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = span[j * kL + sl];
 }
 
 }  // namespace dev

@@ -56,6 +56,7 @@ struct RmsNormArgs {
     int64_t rows = 0;
     int O = 0;
     MxView out;
+    bool vec_q = false;  // out's rows are aligned to the stores of eight elements (set by the launcher)
     float* inv_rms = nullptr;
 };
 cudaError_t add_rms_norm(const RmsNormArgs& a, cudaStream_t st);

@@ -31,13 +31,14 @@ struct Divisor {
     __device__ int operator()(int i) const { return int((uint64_t(uint32_t(i)) * m) >> shift); }
 };
 
-// A launch covers rows whose work numbers fit 31 bits. Aligned rows of whole groups of eight columns: a
-// number is (row, group), padded to whole blocks of four groups, and a thread takes two of them half the work
-// apart, so that two loads are in flight. Every other layout: a number is (row, block) and a warp's, one
-// column per lane, so that its loads and stores stay coalesced.
+// A launch covers rows whose work numbers fit 31 bits. A number is (row, group of eight columns), padded to whole
+// spans of kL groups. Aligned rows (O a multiple of 8): kL = 4, a block, and a thread takes two groups half the work
+// apart, so that two loads are in flight. Every other layout: kL (4 .. 32, a row's groups at most) neighbouring
+// threads deal a span's columns out over them for coalesced single accesses, and turn them in shared memory.
 struct Shape {
     int rows, O, per_row, half;  // numbers of a row; numbers of a thread's first part
     Divisor by_row;
+    bool vec_q;                  // Q's rows are aligned to the stores of eight elements
 };
 
 template <typename T>
@@ -58,29 +59,56 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T* __restri
                        Q.s + int64_t(row[k]) * Q.lds + c[k] / kMxBlock, true);
 }
 
-template <typename T>
+template <typename T, int kL>
 __global__ void __launch_bounds__(kThreads) mx_quantize_columns_kernel(const T* __restrict__ X, int64_t ldx, Shape sh, MxView Q) {
-    const int lane = threadIdx.x & 31;
-    float v[4];
-    int row[4], c[4];
+    __shared__ __align__(16) float turn[8 * kThreads];
+    const int sl = threadIdx.x % kL;
+    float t[2][8];
+    int row[2], c[2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int i = (int(blockIdx.x) * (kThreads / 32) + int(threadIdx.x >> 5)) * 4 + k;
+    for (int k = 0; k < 2; ++k) {
+        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.half;
         row[k] = sh.by_row(i);
-        c[k] = kMxBlock * (i - row[k] * sh.per_row) + lane;
-        if (row[k] >= sh.rows) c[k] = sh.O;
-        v[k] = c[k] < sh.O ? to_f32(X[int64_t(row[k]) * ldx + c[k]]) : 0.f;
+        c[k] = 8 * (i - row[k] * sh.per_row);
+        if (i - k * sh.half >= sh.half || row[k] >= sh.rows) c[k] = sh.O + 8 * sl;  // nothing exists
+        const int first = c[k] - 8 * sl;
+        const T* p = X + int64_t(row[k]) * ldx + first + sl;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[k][j] = first + j * kL + sl < sh.O ? to_f32(p[j * kL]) : 0.f;
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        mx_store_column(v[k], c[k] < sh.O, c[k] + 1 < sh.O, Q.q4, Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]),
-                        Q.s + int64_t(row[k]) * Q.lds + c[k] / kMxBlock);
+    for (int k = 0; k < 2; ++k) {
+        float v[8];
+        turn_to_groups<kL>(t[k], v, turn + 8 * (threadIdx.x - sl), sl);
+        mx_store_block(v, max(0, min(8, sh.O - c[k])), Q.q4, Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]),
+                       Q.s + int64_t(row[k]) * Q.lds + c[k] / kMxBlock, sh.vec_q);
+    }
+}
+
+// Eight elements from byte q on as fp32, times their block's scale; nv of them exist.
+__device__ __forceinline__ void decode8(const uint8_t* q, const uint8_t* s, bool q4, int nv, bool vec, float (&v)[8]) {
+    uint32_t w[2] = {0u, 0u};
+    if (vec && nv == 8) {
+        if (q4) w[0] = __ldcs(reinterpret_cast<const uint32_t*>(q));
+        else *reinterpret_cast<uint2*>(w) = __ldcs(reinterpret_cast<const uint2*>(q));
+    } else {
+        const int bytes = q4 ? (nv + 1) / 2 : nv;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < bytes) w[k >> 2] |= uint32_t(q[k]) << (8 * (k & 3));
+    }
+    const float scale = nv > 0 ? mx_scale_value(*s) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = mx_f16x2_to_f32(q4 ? mx_decode2_e2m1((w[0] >> (8 * j)) & 0xffu) : mx_decode2_e4m3((w[j >> 1] >> (16 * (j & 1))) & 0xffffu));
+        v[2 * j] = f.x * scale;
+        v[2 * j + 1] = f.y * scale;
+    }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(MxView Q, Shape sh, T* __restrict__ Y, int64_t ldy) {
-    uint32_t w[2][2];
-    float scale[2];
+    float v[2][8];
     int row[2], c[2];
     bool live[2];
 #pragma unroll
@@ -89,48 +117,38 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(MxView Q, Shape
         row[k] = sh.by_row(i);
         c[k] = 8 * (i - row[k] * sh.per_row);
         live[k] = i - k * sh.half < sh.half && row[k] < sh.rows && c[k] < sh.O;
-        if (!live[k]) continue;
-        const uint8_t* q = Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]);
-        if (Q.q4) w[k][0] = __ldcs(reinterpret_cast<const uint32_t*>(q));
-        else *reinterpret_cast<uint2*>(w[k]) = __ldcs(reinterpret_cast<const uint2*>(q));
-        scale[k] = mx_scale_value(Q.s[int64_t(row[k]) * Q.lds + c[k] / kMxBlock]);
+        if (live[k])
+            decode8(Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]), Q.s + int64_t(row[k]) * Q.lds + c[k] / kMxBlock, Q.q4, 8, true, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (live[k]) store8(Y + int64_t(row[k]) * ldy + c[k], 8, true, v[k]);
+}
+
+template <typename T, int kL>
+__global__ void __launch_bounds__(kThreads) mx_dequantize_columns_kernel(MxView Q, Shape sh, T* __restrict__ Y, int64_t ldy) {
+    __shared__ __align__(16) float turn[8 * kThreads];
+    const int sl = threadIdx.x % kL;
+    float v[2][8];
+    int row[2], c[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.half;
+        row[k] = sh.by_row(i);
+        c[k] = 8 * (i - row[k] * sh.per_row);
+        if (i - k * sh.half >= sh.half || row[k] >= sh.rows) c[k] = sh.O + 8 * sl;  // nothing exists
+        decode8(Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]), Q.s + int64_t(row[k]) * Q.lds + c[k] / kMxBlock, Q.q4,
+                max(0, min(8, sh.O - c[k])), sh.vec_q, v[k]);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        if (!live[k]) continue;
-        float v[8];
+        float t[8];
+        turn_to_columns<kL>(v[k], t, turn + 8 * (threadIdx.x - sl), sl);
+        const int first = c[k] - 8 * sl;
+        T* p = Y + int64_t(row[k]) * ldy + first + sl;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = mx_f16x2_to_f32(Q.q4 ? mx_decode2_e2m1((w[k][0] >> (8 * j)) & 0xffu)
-                                                  : mx_decode2_e4m3((w[k][j >> 1] >> (16 * (j & 1))) & 0xffffu));
-            v[2 * j] = f.x * scale[k];
-            v[2 * j + 1] = f.y * scale[k];
-        }
-        store8(Y + int64_t(row[k]) * ldy + c[k], 8, true, v);
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) mx_dequantize_columns_kernel(MxView Q, Shape sh, T* __restrict__ Y, int64_t ldy) {
-    const int lane = threadIdx.x & 31;
-    uint32_t w[4];
-    float scale[4];
-    int row[4], c[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int i = (int(blockIdx.x) * (kThreads / 32) + int(threadIdx.x >> 5)) * 4 + k;
-        row[k] = sh.by_row(i);
-        c[k] = kMxBlock * (i - row[k] * sh.per_row) + lane;
-        if (row[k] >= sh.rows) c[k] = sh.O;
-        if (c[k] >= sh.O) continue;
-        w[k] = Q.q[int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k])];
-        scale[k] = mx_scale_value(Q.s[int64_t(row[k]) * Q.lds + c[k] / kMxBlock]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        if (c[k] >= sh.O) continue;
-        const float2 f = mx_f16x2_to_f32(Q.q4 ? mx_decode2_e2m1(w[k]) : mx_decode2_e4m3(w[k]));
-        Y[int64_t(row[k]) * ldy + c[k]] = from_f32<T>((Q.q4 && (c[k] & 1) ? f.y : f.x) * scale[k]);
+        for (int j = 0; j < 8; ++j)
+            if (first + j * kL + sl < sh.O) p[j * kL] = from_f32<T>(t[j]);
     }
 }
 
@@ -138,20 +156,21 @@ bool rows_aligned(const void* p, int64_t ld_bytes, int64_t bytes) {
     return reinterpret_cast<uintptr_t>(p) % uintptr_t(bytes) == 0 && ld_bytes % bytes == 0;
 }
 
-// Calls launch(first row, shape, blocks, whole groups?) for slices of rows whose work numbers fit 31 bits.
+// Calls launch(first row, shape, blocks, lanes) for slices of rows whose work numbers fit 31 bits; lanes = 0: aligned
+// rows, else the kL of the other form.
 template <typename T, class Fn>
 cudaError_t sliced(const DenseView& X, int64_t rows, int O, const MxView& Q, Fn&& launch) {
-    const int blocks = (O + kMxBlock - 1) / kMxBlock;
-    const bool groups = O % 8 == 0 && rows_aligned(X.p, X.ld * int64_t(sizeof(T)), 16) && rows_aligned(Q.q, Q.ldq, Q.q4 ? 4 : 8);
-    const int per_row = groups ? 4 * blocks : blocks;
+    const bool vec_q = rows_aligned(Q.q, Q.ldq, Q.q4 ? 4 : 8);
+    const bool vec = O % 8 == 0 && rows_aligned(X.p, X.ld * int64_t(sizeof(T)), 16) && vec_q;
+    int span = 4;  // groups of eight columns
+    if (!vec)
+        while (span < 32 && 8 * span < O) span *= 2;
+    const int per_row = (O + 8 * span - 1) / (8 * span) * span;
     const int64_t most = std::max<int64_t>(1, int64_t(0x7ff00000) / per_row);
     for (int64_t r = 0; r < rows; r += most) {
         const int64_t n = std::min(most, rows - r);
-        const int64_t numbers = n * per_row;
-        const int64_t per_block = groups ? kThreads : kThreads / 32 * 4;
-        const int64_t half = (numbers / 4 + 1) / 2 * 4;  // whole blocks of four groups
-        const int64_t grid = ((groups ? half : numbers) + per_block - 1) / per_block;
-        launch(r, Shape{int(n), O, per_row, int(half), Divisor(per_row)}, unsigned(grid), groups);
+        const int64_t half = (n * per_row / span + 1) / 2 * span;  // whole spans
+        launch(r, Shape{int(n), O, per_row, int(half), Divisor(per_row), vec_q}, unsigned((half + kThreads - 1) / kThreads), vec ? 0 : span);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
     }
@@ -166,19 +185,27 @@ MxView from_row(MxView Q, int64_t r) {
 
 template <typename T>
 cudaError_t quantize_t(const DenseView& X, int64_t rows, int O, const MxView& Q, cudaStream_t st) {
-    return sliced<T>(X, rows, O, Q, [&](int64_t r, const Shape& sh, unsigned blocks, bool groups) {
+    return sliced<T>(X, rows, O, Q, [&](int64_t r, const Shape& sh, unsigned blocks, int lanes) {
         const T* x = static_cast<const T*>(X.p) + r * X.ld;
-        if (groups) mx_quantize_kernel<T><<<blocks, kThreads, 0, st>>>(x, X.ld, sh, from_row(Q, r));
-        else mx_quantize_columns_kernel<T><<<blocks, kThreads, 0, st>>>(x, X.ld, sh, from_row(Q, r));
+        const MxView q = from_row(Q, r);
+        if (lanes == 0) mx_quantize_kernel<T><<<blocks, kThreads, 0, st>>>(x, X.ld, sh, q);
+        else if (lanes == 4) mx_quantize_columns_kernel<T, 4><<<blocks, kThreads, 0, st>>>(x, X.ld, sh, q);
+        else if (lanes == 8) mx_quantize_columns_kernel<T, 8><<<blocks, kThreads, 0, st>>>(x, X.ld, sh, q);
+        else if (lanes == 16) mx_quantize_columns_kernel<T, 16><<<blocks, kThreads, 0, st>>>(x, X.ld, sh, q);
+        else mx_quantize_columns_kernel<T, 32><<<blocks, kThreads, 0, st>>>(x, X.ld, sh, q);
     });
 }
 
 template <typename T>
 cudaError_t dequantize_t(const MxView& Q, int64_t rows, int O, const DenseView& Y, cudaStream_t st) {
-    return sliced<T>(Y, rows, O, Q, [&](int64_t r, const Shape& sh, unsigned blocks, bool groups) {
+    return sliced<T>(Y, rows, O, Q, [&](int64_t r, const Shape& sh, unsigned blocks, int lanes) {
         T* y = static_cast<T*>(Y.p) + r * Y.ld;
-        if (groups) mx_dequantize_kernel<T><<<blocks, kThreads, 0, st>>>(from_row(Q, r), sh, y, Y.ld);
-        else mx_dequantize_columns_kernel<T><<<blocks, kThreads, 0, st>>>(from_row(Q, r), sh, y, Y.ld);
+        const MxView q = from_row(Q, r);
+        if (lanes == 0) mx_dequantize_kernel<T><<<blocks, kThreads, 0, st>>>(q, sh, y, Y.ld);
+        else if (lanes == 4) mx_dequantize_columns_kernel<T, 4><<<blocks, kThreads, 0, st>>>(q, sh, y, Y.ld);
+        else if (lanes == 8) mx_dequantize_columns_kernel<T, 8><<<blocks, kThreads, 0, st>>>(q, sh, y, Y.ld);
+        else if (lanes == 16) mx_dequantize_columns_kernel<T, 16><<<blocks, kThreads, 0, st>>>(q, sh, y, Y.ld);
+        else mx_dequantize_columns_kernel<T, 32><<<blocks, kThreads, 0, st>>>(q, sh, y, Y.ld);
     });
 }
 

@@ -10,29 +10,34 @@ namespace vcsrmc {
 namespace dev {
 namespace {
 
-// dweight[c] = sum over the blocks' partial rows: 32 columns per block, 8 warps over the rows, four in flight.
-__global__ void __launch_bounds__(256) rms_norm_dweight_kernel(const float* __restrict__ part, int n, int O, float* __restrict__ dw) {
-    __shared__ float s[8][32];
+// dweight[c] = sum over the blocks' partial rows: 32 columns per block, 32 warps over the rows, eight in flight. (Eight
+// warps with four in flight took half of the backward pass of 8192 rows of 1000.)
+constexpr int kSumWarps = 32, kSumFlight = 8;
+__global__ void __launch_bounds__(kSumWarps * 32) rms_norm_dweight_kernel(const float* __restrict__ part, int n, int O, float* __restrict__ dw) {
+    __shared__ float s[kSumWarps][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = int(blockIdx.x) * 32 + lane;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    float v[kSumFlight] = {};
     wait_for_launch_before();  // the partial sums
     if (c < O) {
-        int i = warp;
-        for (; i + 24 < n; i += 32) {
+        for (int i = warp; i < n; i += kSumWarps * kSumFlight) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] += part[int64_t(i + 8 * k) * O + c];
+            for (int k = 0; k < kSumFlight; ++k)
+                if (i + k * kSumWarps < n) v[k] += part[int64_t(i + k * kSumWarps) * O + c];
         }
-        for (; i < n; i += 8) v[0] += part[int64_t(i) * O + c];
     }
-    s[warp][lane] = (v[0] + v[1]) + (v[2] + v[3]);
-    __syncthreads();
-    if (warp == 0 && c < O) {
-        float t = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) t += s[k][lane];
-        dw[c] = t;
-    }
+    for (int d = 1; d < kSumFlight; d *= 2)
+#pragma unroll
+        for (int k = 0; k < kSumFlight; k += 2 * d) v[k] += v[k + d];
+    s[warp][lane] = v[0];
+    __syncthreads();
+    // warp w adds up column w's 32 sums
+    float t = s[lane][warp];
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+    const int column = int(blockIdx.x) * 32 + warp;
+    if (lane == 0 && column < O) dw[column] = t;
 }
 
 // Blocks of the backward pass: enough to fill every SM with about 1024 threads, or one for every row (or
@@ -53,6 +58,7 @@ int64_t grad_blocks(int64_t rows, int O, int sms) {
 cudaError_t add_rms_norm(const RmsNormArgs& args, cudaStream_t st) {
     RmsNormArgs a = args;
     a.vec_w = reinterpret_cast<uintptr_t>(a.weight) % 16 == 0;
+    a.vec_q = norm::aligned(a.out.q, a.out.ldq, a.out.q4 ? 4 : 8);
     if (a.x.dtype != VCSRMC_F32) return norm::forward<false, false>(a, st);
     return a.residual_out.dtype == VCSRMC_F32 ? norm::forward<true, true>(a, st) : norm::forward<true, false>(a, st);
 }
@@ -67,7 +73,7 @@ cudaError_t add_rms_norm_backward(const RmsNormGradArgs& args, int sms, cudaStre
                           : a.hidden.dtype == VCSRMC_F32 ? norm::backward<true, true>(a, blocks, st)
                                                          : norm::backward<true, false>(a, blocks, st);
     if (e != cudaSuccess) return e;
-    LaunchAfter L(dim3(unsigned((a.O + 31) / 32), 1, 1), dim3(256, 1, 1), st);
+    LaunchAfter L(dim3(unsigned((a.O + 31) / 32), 1, 1), dim3(kSumWarps * 32, 1, 1), st);
     return cudaLaunchKernelEx(&L.cfg, rms_norm_dweight_kernel, static_cast<const float*>(a.workspace), int(blocks), a.O, a.dweight);
 }
 

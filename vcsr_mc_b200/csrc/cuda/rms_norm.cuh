@@ -25,25 +25,29 @@ namespace vcsrmc {
 namespace dev {
 namespace norm {
 
-// How a row lies over threads. kV = 8: a thread holds groups of eight consecutive columns (16-byte loads and
-// stores; O is a multiple of 8 and every row aligned), kV = 1: single columns, neighbouring threads
-// neighbouring columns, for every other layout. kN columns per thread in all, on kL lanes of a warp or, for
-// kL = 0, on the whole block. kN = 0: any width in steps of 8, the row is read twice.
+// How a row lies over threads: kN columns per thread, in groups of eight, on kL lanes of a warp or, for kL = 0, on
+// the whole block. kN = 0: any width in steps of 8, the row is read twice. kV = 8: a group is eight consecutive
+// columns (16-byte loads and stores; O is a multiple of 8 and every row aligned). kV = 1, for every other layout:
+// the columns of neighbouring threads' groups are dealt out over them in turn, so that single loads and stores are
+// coalesced; a block of scales needs them turned into consecutive ones (turn_to_groups).
 template <int kV_, int kL_, int kN_, int kThreads_ = 256>
 struct Span {
     static constexpr int kV = kV_, kL = kL_;
     static constexpr bool kAny = kN_ == 0;
-    static constexpr int kN = kAny ? 8 : kN_;  // columns held at once
+    static constexpr int kN = kAny ? 8 : kN_;      // columns held at once
     static constexpr int kThreads = kThreads_;     // per block, at most
     static constexpr int kRows = kL_ ? 256 / (kL_ ? kL_ : 1) : 1;  // rows in a block
-    static_assert(kN % kV == 0 && (kV == 8 || kL == 0 || kL == 32), "whole groups; single columns on whole warps");
+    static constexpr int kW = kL_ ? kL_ : 32;      // threads whose groups are neighbours
+    static_assert(kN % 8 == 0, "whole groups");
     __device__ static int per_row() { return kL ? kL : int(blockDim.x); }
     __device__ static int slot() { return kL ? int(threadIdx.x) % (kL ? kL : 1) : int(threadIdx.x); }
     __device__ static int row_in_block() { return kL ? int(threadIdx.x) / (kL ? kL : 1) : 0; }
-    // column of this thread's element i, `step` kN-wide steps into the row
+    // first column of this thread's group g, `step` kN-wide steps into the row
+    __device__ static int group(int g, int step = 0) { return 8 * ((step * (kN / 8) + g) * per_row() + slot()); }
+    // column of its element i
     __device__ static int column(int i, int step = 0) {
-        const int at = step * (kN / kV) + i / kV;
-        return kV * (at * per_row() + slot()) + i % kV;
+        if (kV == 8) return group(i / 8, step) + i % 8;
+        return group(i / 8, step) - 8 * (slot() % kW) + (i % 8) * kW + slot() % kW;
     }
 };
 
@@ -172,6 +176,7 @@ __device__ __forceinline__ float inverse_root(double v) {
 template <class S, bool kXWide, bool kRWide>
 __global__ void __launch_bounds__(S::kThreads) rms_norm_kernel(RmsNormArgs a) {
     __shared__ double smem[32];
+    extern __shared__ __align__(16) float turn[];  // kV = 1: eight floats a thread
     const int64_t row = int64_t(blockIdx.x) * S::kRows + S::row_in_block();
     const bool live = row < a.rows;  // every thread takes part in the reductions of a row past the end
     const int O = live ? a.O : 0;
@@ -214,16 +219,16 @@ __global__ void __launch_bounds__(S::kThreads) rms_norm_kernel(RmsNormArgs a) {
         float w[S::kN];
         load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, O, k);
 #pragma unroll
-        for (int i = 0; i < S::kN; i += S::kV) {
-            const int c = S::column(i, k);
-            if constexpr (S::kV == 8) {
-                float y[8];
+        for (int i = 0; i < S::kN; i += 8) {
+            float y[8], t[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = s[i + j] * inv * w[i + j];
-                mx_store_block(y, c < O ? 8 : 0, a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock, true);
+            for (int j = 0; j < 8; ++j) t[j] = s[i + j] * inv * w[i + j];
+            const int c = S::group(i / 8, k);
+            if constexpr (S::kV == 1) {
+                turn_to_groups<S::kW>(t, y, turn + 8 * (threadIdx.x - S::slot() % S::kW), S::slot() % S::kW);
+                mx_store_block(y, max(0, min(8, O - c)), a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock, a.vec_q);
             } else {
-                const float y = s[i] * inv * w[i];
-                mx_store_column(y, c < O, c + 1 < O, a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock);
+                mx_store_block(t, c < O ? 8 : 0, a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock, true);
             }
         }
     }
@@ -242,51 +247,71 @@ __global__ void __launch_bounds__(S::kThreads, S::kL ? 4 : 2) rms_norm_grad_kern
     float* part = a.workspace + int64_t(blockIdx.x) * a.O;
     float dw[S::kN] = {}, w[S::kN];
     if constexpr (!S::kAny) load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, a.O);
-    for (int64_t r0 = int64_t(blockIdx.x) * S::kRows; r0 < a.rows; r0 += int64_t(gridDim.x) * S::kRows) {
-        const int64_t row = r0 + S::row_in_block();
-        const bool live = row < a.rows;
-        const int O = live ? a.O : 0;
-        Held<S, kYWide> dy;
-        Held<S, kRWide> h, dr;
-        const float inv = live ? a.inv_rms[row] : 0.f;
-        auto load_step = [&](int k) {
-            load(dy, a.dy, row, O, k);
-            load(h, a.hidden, row, O, k);
-            if constexpr (S::kAny) load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, O, k);
-        };
+    const int64_t stride = int64_t(gridDim.x) * S::kRows;
+    Held<S, kYWide> dy;
+    Held<S, kRWide> h, dr;
+    float inv = 0.f;
+    // the inputs of a row's step; rows past the end read nothing and count as zeros
+    auto load_row = [&](int64_t row, int k, bool residual) {
+        const int O = row < a.rows ? a.O : 0;
+        inv = row < a.rows ? a.inv_rms[row] : 0.f;
+        load(dy, a.dy, row, O, k);
+        load(h, a.hidden, row, O, k);
+        if (residual && a.d_residual.p) load(dr, a.d_residual, row, O, k);
+    };
+    int64_t row = int64_t(blockIdx.x) * S::kRows + S::row_in_block();
+    // a block's row: the next row's inputs are loaded over this one's reduction and stores (rows of 4096: 189
+    // against 235 us); warps' rows overlap one another, and the registers would cost more (rows of 128: 334
+    // against 236 us)
+    constexpr bool kAhead = !S::kAny && S::kL == 0;
+    if constexpr (kAhead) load_row(row, 0, true);
+    for (int64_t r0 = int64_t(blockIdx.x) * S::kRows; r0 < a.rows; r0 += stride, row += stride) {
+        const int O = row < a.rows ? a.O : 0;
+        float vy[S::kN], vh[S::kN], dx[S::kN] = {};
         // the gradient g = dy * w is 0 past the row's end, where w is, and so are its products
         float dot = 0.f;
         for (int k = 0; k < steps; ++k) {
-            load_step(k);
-            if (!S::kAny && a.d_residual.p) load(dr, a.d_residual, row, O);
-            float vy[S::kN], vh[S::kN];
+            if constexpr (!kAhead) load_row(row, k, !S::kAny);
+            if constexpr (S::kAny) load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, O, k);
             to_floats(dy, a.dy.dtype, vy);
             to_floats(h, a.hidden.dtype, vh);
 #pragma unroll
-            for (int i = 0; i < S::kN; ++i) dot = fmaf(vy[i] * w[i], vh[i] * inv, dot);
+            for (int i = 0; i < S::kN; ++i) {
+                vh[i] *= inv;
+                dot = fmaf(vy[i] * w[i], vh[i], dot);
+            }
+        }
+        const float inv_row = inv;
+        if constexpr (kAhead) {
+            if (a.d_residual.p) to_floats(dr, a.hidden.dtype, dx);
+            load_row(row + stride, 0, true);
         }
         const float m = row_sum<S>(dot, smem) / float(a.O);
         for (int k = 0; k < steps; ++k) {
             if constexpr (S::kAny) {
-                load_step(k);
-                if (a.d_residual.p) load(dr, a.d_residual, row, O, k);
+                load_row(row, k, true);
+                load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, O, k);
+                to_floats(dy, a.dy.dtype, vy);
+                to_floats(h, a.hidden.dtype, vh);
+#pragma unroll
+                for (int i = 0; i < S::kN; ++i) vh[i] *= inv;
             }
-            float vy[S::kN], vh[S::kN], dx[S::kN] = {};
-            to_floats(dy, a.dy.dtype, vy);
-            to_floats(h, a.hidden.dtype, vh);
-            if (a.d_residual.p) to_floats(dr, a.hidden.dtype, dx);
+            if (!kAhead && a.d_residual.p) to_floats(dr, a.hidden.dtype, dx);
 #pragma unroll
             for (int i = 0; i < S::kN; ++i) {
-                const float n = vh[i] * inv;
-                dx[i] = fmaf(inv, fmaf(vy[i], w[i], -(n * m)), dx[i]);
+                dx[i] = fmaf(inv_row, fmaf(vy[i], w[i], -(vh[i] * m)), dx[i]);
                 if constexpr (S::kAny) {
                     const int c = S::column(i, k);
-                    if (c < O) part[c] = fmaf(vy[i], n, r0 == int64_t(blockIdx.x) ? 0.f : part[c]);
+                    if (c < O) part[c] = fmaf(vy[i], vh[i], r0 == int64_t(blockIdx.x) ? 0.f : part[c]);
                 } else {
-                    dw[i] = fmaf(vy[i], n, dw[i]);
+                    dw[i] = fmaf(vy[i], vh[i], dw[i]);
                 }
             }
             store<S, kRWide>(dx, a.dx, row, O, k);
+            if constexpr (S::kAny) {
+#pragma unroll
+                for (int i = 0; i < S::kN; ++i) dx[i] = 0.f;
+            }
         }
     }
     if constexpr (!S::kAny && S::kL > 0) {
@@ -295,13 +320,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kL ? 4 : 2) rms_norm_grad_kern
         for (int i0 = 0; i0 < S::kN; i0 += 8) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8 && i0 + i < S::kN; ++i) fold[i][threadIdx.x] = dw[i0 + i];
+            for (int i = 0; i < 8; ++i) fold[i][threadIdx.x] = dw[i0 + i];
             __syncthreads();
             for (int t = int(threadIdx.x); t < S::kL * 8; t += 256) {
                 const int i = t / S::kL, slot = t % S::kL;
-                const int at = (i0 + i) / S::kV;
-                const int c = S::kV * (at * S::kL + slot) + (i0 + i) % S::kV;
-                if (i0 + i < S::kN && c < a.O) {
+                const int c = i0 * S::kL + (S::kV == 8 ? 8 * slot + i : i * S::kL + slot);
+                if (c < a.O) {
                     float v = 0.f;
                     for (int g = 0; g < S::kRows; ++g) v += fold[i][g * S::kL + slot];
                     part[c] = v;
@@ -329,7 +353,8 @@ template <class S, bool kXWide, bool kRWide>
 cudaError_t launch_norm(const RmsNormArgs& a, int threads, cudaStream_t st) {
     const int64_t blocks = (a.rows + S::kRows - 1) / S::kRows;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    rms_norm_kernel<S, kXWide, kRWide><<<unsigned(blocks), S::kL ? 256 : threads, 0, st>>>(a);
+    const int n = S::kL ? 256 : threads;
+    rms_norm_kernel<S, kXWide, kRWide><<<unsigned(blocks), n, S::kV == 1 ? 8 * n * sizeof(float) : 0, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -339,55 +364,43 @@ cudaError_t launch_grad(const RmsNormGradArgs& a, int threads, int64_t blocks, c
     return cudaGetLastError();
 }
 
+template <int kV, bool kXWide, bool kRWide>
+cudaError_t forward_spans(const RmsNormArgs& a, cudaStream_t st) {
+    const int O = a.O;
+    if (O <= 32) return launch_norm<Span<kV, 4, 8>, kXWide, kRWide>(a, 0, st);
+    if (O <= 64) return launch_norm<Span<kV, 8, 8>, kXWide, kRWide>(a, 0, st);
+    if (O <= 128) return launch_norm<Span<kV, 16, 8>, kXWide, kRWide>(a, 0, st);
+    if (O <= 256) return launch_norm<Span<kV, 32, 8>, kXWide, kRWide>(a, 0, st);
+    if (O <= 512) return launch_norm<Span<kV, 32, 16>, kXWide, kRWide>(a, 0, st);
+    if (O <= 8 * 1024) return launch_norm<Span<kV, 0, 8, 1024>, kXWide, kRWide>(a, threads_for(O, 8), st);
+    if (O <= 16 * 1024) return launch_norm<Span<kV, 0, 16, 1024>, kXWide, kRWide>(a, threads_for(O, 16), st);
+    return launch_norm<Span<kV, 0, 0, 1024>, kXWide, kRWide>(a, 1024, st);
+}
+
+template <int kV, bool kYWide, bool kRWide>
+cudaError_t backward_spans(const RmsNormGradArgs& a, int64_t blocks, cudaStream_t st) {
+    const int O = a.O, threads = grad_threads(O);
+    if (O <= 32) return launch_grad<Span<kV, 4, 8>, kYWide, kRWide>(a, 0, blocks, st);
+    if (O <= 64) return launch_grad<Span<kV, 8, 8>, kYWide, kRWide>(a, 0, blocks, st);
+    if (O <= 128) return launch_grad<Span<kV, 16, 8>, kYWide, kRWide>(a, 0, blocks, st);
+    if (O <= 256) return launch_grad<Span<kV, 32, 8>, kYWide, kRWide>(a, 0, blocks, st);
+    if (O <= 4096) return launch_grad<Span<kV, 0, 8, 512>, kYWide, kRWide>(a, threads, blocks, st);
+    if (O <= 8192) return launch_grad<Span<kV, 0, 16, 512>, kYWide, kRWide>(a, threads, blocks, st);
+    return launch_grad<Span<kV, 0, 0, 512>, kYWide, kRWide>(a, threads, blocks, st);
+}
+
 // The launches of one pair of element widths (X or dY, residual); each pair is a translation unit.
 template <bool kXWide, bool kRWide>
 cudaError_t forward(const RmsNormArgs& a, cudaStream_t st) {
-    const int O = a.O;
-    const bool vec = O % 8 == 0 && aligned16(a.x) && (!a.residual.p || aligned16(a.residual)) &&
-                     (!a.residual_out.p || aligned16(a.residual_out)) && aligned(a.out.q, a.out.ldq, a.out.q4 ? 4 : 8);
-    if (vec) {
-        if (O <= 32) return launch_norm<Span<8, 4, 8>, kXWide, kRWide>(a, 0, st);
-        if (O <= 64) return launch_norm<Span<8, 8, 8>, kXWide, kRWide>(a, 0, st);
-        if (O <= 128) return launch_norm<Span<8, 16, 8>, kXWide, kRWide>(a, 0, st);
-        if (O <= 256) return launch_norm<Span<8, 32, 8>, kXWide, kRWide>(a, 0, st);
-        if (O <= 512) return launch_norm<Span<8, 32, 16>, kXWide, kRWide>(a, 0, st);
-        if (O <= 1024) return launch_norm<Span<8, 32, 32>, kXWide, kRWide>(a, 0, st);
-        if (O <= 8 * 1024) return launch_norm<Span<8, 0, 8, 1024>, kXWide, kRWide>(a, threads_for(O, 8), st);
-        if (O <= 16 * 1024) return launch_norm<Span<8, 0, 16, 1024>, kXWide, kRWide>(a, threads_for(O, 16), st);
-        return launch_norm<Span<8, 0, 0, 1024>, kXWide, kRWide>(a, 1024, st);
-    }
-    if (O <= 32) return launch_norm<Span<1, 32, 1>, kXWide, kRWide>(a, 0, st);
-    if (O <= 64) return launch_norm<Span<1, 32, 2>, kXWide, kRWide>(a, 0, st);
-    if (O <= 128) return launch_norm<Span<1, 32, 4>, kXWide, kRWide>(a, 0, st);
-    if (O <= 256) return launch_norm<Span<1, 32, 8>, kXWide, kRWide>(a, 0, st);
-    if (O <= 512) return launch_norm<Span<1, 32, 16>, kXWide, kRWide>(a, 0, st);
-    if (O <= 1024) return launch_norm<Span<1, 32, 32>, kXWide, kRWide>(a, 0, st);
-    if (O <= 8 * 1024) return launch_norm<Span<1, 0, 8, 1024>, kXWide, kRWide>(a, threads_for(O, 8), st);
-    if (O <= 16 * 1024) return launch_norm<Span<1, 0, 16, 1024>, kXWide, kRWide>(a, threads_for(O, 16), st);
-    return launch_norm<Span<1, 0, 0, 1024>, kXWide, kRWide>(a, 1024, st);
+    const bool vec = a.O % 8 == 0 && aligned16(a.x) && (!a.residual.p || aligned16(a.residual)) &&
+                     (!a.residual_out.p || aligned16(a.residual_out)) && a.vec_q;
+    return vec ? forward_spans<8, kXWide, kRWide>(a, st) : forward_spans<1, kXWide, kRWide>(a, st);
 }
 
 template <bool kYWide, bool kRWide>
 cudaError_t backward(const RmsNormGradArgs& a, int64_t blocks, cudaStream_t st) {
-    const int O = a.O;
-    const bool vec = O % 8 == 0 && aligned16(a.dy) && aligned16(a.hidden) && aligned16(a.dx) && (!a.d_residual.p || aligned16(a.d_residual));
-    const int threads = grad_threads(O);
-    if (vec) {
-        if (O <= 32) return launch_grad<Span<8, 4, 8>, kYWide, kRWide>(a, 0, blocks, st);
-        if (O <= 64) return launch_grad<Span<8, 8, 8>, kYWide, kRWide>(a, 0, blocks, st);
-        if (O <= 128) return launch_grad<Span<8, 16, 8>, kYWide, kRWide>(a, 0, blocks, st);
-        if (O <= 256) return launch_grad<Span<8, 32, 8>, kYWide, kRWide>(a, 0, blocks, st);
-        if (O <= 4096) return launch_grad<Span<8, 0, 8, 512>, kYWide, kRWide>(a, threads, blocks, st);
-        if (O <= 8192) return launch_grad<Span<8, 0, 16, 512>, kYWide, kRWide>(a, threads, blocks, st);
-        return launch_grad<Span<8, 0, 0, 512>, kYWide, kRWide>(a, threads, blocks, st);
-    }
-    if (O <= 32) return launch_grad<Span<1, 32, 1>, kYWide, kRWide>(a, 0, blocks, st);
-    if (O <= 64) return launch_grad<Span<1, 32, 2>, kYWide, kRWide>(a, 0, blocks, st);
-    if (O <= 128) return launch_grad<Span<1, 32, 4>, kYWide, kRWide>(a, 0, blocks, st);
-    if (O <= 256) return launch_grad<Span<1, 32, 8>, kYWide, kRWide>(a, 0, blocks, st);
-    if (O <= 4096) return launch_grad<Span<1, 0, 8, 512>, kYWide, kRWide>(a, threads, blocks, st);
-    if (O <= 8192) return launch_grad<Span<1, 0, 16, 512>, kYWide, kRWide>(a, threads, blocks, st);
-    return launch_grad<Span<1, 0, 0, 512>, kYWide, kRWide>(a, threads, blocks, st);
+    const bool vec = a.O % 8 == 0 && aligned16(a.dy) && aligned16(a.hidden) && aligned16(a.dx) && (!a.d_residual.p || aligned16(a.d_residual));
+    return vec ? backward_spans<8, kYWide, kRWide>(a, blocks, st) : backward_spans<1, kYWide, kRWide>(a, blocks, st);
 }
 
 extern template cudaError_t forward<true, true>(const RmsNormArgs&, cudaStream_t);
