@@ -32,17 +32,6 @@ __device__ __forceinline__ float mx_scale_value(uint32_t code) {
     return __uint_as_float(code == kMxNan ? 0x7fffffffu : bits);
 }
 
-// Two elements, `lo` in the low half of the result (8 bits of it for E2M1, 16 for E4M3).
-__device__ __forceinline__ uint32_t mx_encode2_e2m1(float lo, float hi) {
-    uint32_t r;
-    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ uint32_t mx_encode2_e4m3(float lo, float hi) {
-    unsigned short r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
-    return r;
-}
 // Two elements as f16x2 (exact), the low half of the input first.
 __device__ __forceinline__ uint32_t mx_decode2_e2m1(uint32_t byte) {
     uint32_t r;
@@ -122,27 +111,34 @@ __device__ __forceinline__ void store8(T* p, int nv, bool vec, const float (&v)[
     }
 }
 
+// Largest |x| of the two and `m`; a NaN wins.
+__device__ __forceinline__ float max3_abs(float m, float x, float y) {
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(x), "f"(y));
+    return m;
+}
+
 // Quantises and stores eight columns of a block held by four neighbouring lanes (8 columns each; all
 // 32 lanes of the warp take part). `q` is the eight columns' place in the row (byte c for E4M3, c / 2 for
-// E2M1), `s` the block's scale; nv of the eight columns exist (0: nothing is stored). `vec`: q is
-// aligned to its full store (8 bytes for E4M3, 4 for E2M1).
+// E2M1), `s` the block's scale; nv of the eight columns exist (0: nothing is stored), the others are zeros.
+// `vec`: q is aligned to its full store (8 bytes for E4M3, 4 for E2M1).
 __device__ __forceinline__ void mx_store_block(const float (&y)[8], int nv, bool q4, uint8_t* q, uint8_t* s, bool vec) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, i < nv ? __float_as_uint(y[i]) & 0x7fffffffu : 0u);
+    uint32_t amax = __float_as_uint(max3_abs(max3_abs(max3_abs(max3_abs(0.f, y[0], y[1]), y[2], y[3]), y[4], y[5]), y[6], y[7]));
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const uint32_t code = mx_scale_code(amax, q4);
-    const float inv = code == kMxNan ? 0.f : mx_inverse_scale(code);
-    float t[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = code == kMxNan || i >= nv ? 0.f : y[i] * inv;
     if (nv <= 0) return;
+    const uint32_t code = mx_scale_code(amax, q4);
     if ((threadIdx.x & 3) == 0) *s = uint8_t(code);
+    const float inv = mx_inverse_scale(code);  // of no use in a block with the NaN scale
     if (q4) {
         uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w |= mx_encode2_e2m1(t[2 * i], t[2 * i + 1]) << (8 * i);
+        if (code != kMxNan)
+            asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+                "mov.b32 %0, {a, b, c, d};\n\t}"
+                : "=r"(w)
+                : "f"(y[0] * inv), "f"(y[1] * inv), "f"(y[2] * inv), "f"(y[3] * inv), "f"(y[4] * inv), "f"(y[5] * inv), "f"(y[6] * inv),
+                  "f"(y[7] * inv));
         if (vec && nv == 8) {
             *reinterpret_cast<uint32_t*>(q) = w;
         } else {
@@ -151,10 +147,15 @@ __device__ __forceinline__ void mx_store_block(const float (&y)[8], int nv, bool
                 if (2 * i < nv) q[i] = uint8_t(w >> (8 * i));
         }
     } else {
-        uint32_t w[2];
+        uint32_t w[2] = {0u, 0u};
+        if (code != kMxNan) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            w[i] = mx_encode2_e4m3(t[4 * i], t[4 * i + 1]) | (mx_encode2_e4m3(t[4 * i + 2], t[4 * i + 3]) << 16);
+            for (int i = 0; i < 2; ++i)
+                asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
+                    "mov.b32 %0, {a, b};\n\t}"
+                    : "=r"(w[i])
+                    : "f"(y[4 * i] * inv), "f"(y[4 * i + 1] * inv), "f"(y[4 * i + 2] * inv), "f"(y[4 * i + 3] * inv));
+        }
         if (vec && nv == 8) {
             *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
         } else {

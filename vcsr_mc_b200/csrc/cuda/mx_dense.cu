@@ -16,6 +16,8 @@ namespace dev {
 namespace {
 
 constexpr int kThreads = 256;
+// Groups of a thread: reading 4-bit elements takes four to have as much in flight as two of a dense type.
+constexpr int kQuantizeParts = 2, kDequantizeParts = 4;
 
 // i / d for 0 <= i < 2^31 by a multiplication: m = ceil(2^(31 + bits) / d) with 2^(bits - 1) < d <= 2^bits.
 // m * d - 2^(31 + bits) < d <= 2^bits, so i * m / 2^(31 + bits) is above i / d by less than 1 / d.
@@ -32,29 +34,29 @@ struct Divisor {
 };
 
 // A launch covers rows whose work numbers fit 31 bits. A number is (row, group of eight columns), padded to whole
-// spans of kL groups. Aligned rows (O a multiple of 8): kL = 4, a block, and a thread takes two groups half the work
-// apart, so that two loads are in flight. Every other layout: kL (4 .. 32, a row's groups at most) neighbouring
-// threads deal a span's columns out over them for coalesced single accesses, and turn them in shared memory.
+// spans of kL groups; a thread takes kParts of them, `part` apart, so that as many loads are in flight. Aligned rows
+// (O a multiple of 8): kL = 4, a block. Every other layout: kL (4 .. 32, a row's groups at most) neighbouring threads
+// deal a span's columns out over them for coalesced single accesses, and turn them in shared memory.
 struct Shape {
-    int rows, O, per_row, half;  // numbers of a row; numbers of a thread's first part
+    int rows, O, per_row, part;  // per_row: numbers of a row
     Divisor by_row;
     bool vec_q;                  // Q's rows are aligned to the stores of eight elements
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T* __restrict__ X, int64_t ldx, Shape sh, MxView Q) {
-    float v[2][8];
-    int row[2], c[2], nv[2];
+__global__ void __launch_bounds__(kThreads, 8) mx_quantize_kernel(const T* __restrict__ X, int64_t ldx, Shape sh, MxView Q) {
+    float v[kQuantizeParts][8];
+    int row[kQuantizeParts], c[kQuantizeParts], nv[kQuantizeParts];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.half;
+    for (int k = 0; k < kQuantizeParts; ++k) {
+        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.part;
         row[k] = sh.by_row(i);
         c[k] = 8 * (i - row[k] * sh.per_row);
-        nv[k] = i - k * sh.half < sh.half && row[k] < sh.rows && c[k] < sh.O ? 8 : 0;
+        nv[k] = i - k * sh.part < sh.part && row[k] < sh.rows && c[k] < sh.O ? 8 : 0;
         load8(X + int64_t(row[k]) * ldx + c[k], nv[k], true, v[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < kQuantizeParts; ++k)
         mx_store_block(v[k], nv[k], Q.q4, Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]),
                        Q.s + int64_t(row[k]) * Q.lds + c[k] / kMxBlock, true);
 }
@@ -63,21 +65,21 @@ template <typename T, int kL>
 __global__ void __launch_bounds__(kThreads) mx_quantize_columns_kernel(const T* __restrict__ X, int64_t ldx, Shape sh, MxView Q) {
     __shared__ __align__(16) float turn[8 * kThreads];
     const int sl = threadIdx.x % kL;
-    float t[2][8];
-    int row[2], c[2];
+    float t[kQuantizeParts][8];
+    int row[kQuantizeParts], c[kQuantizeParts];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.half;
+    for (int k = 0; k < kQuantizeParts; ++k) {
+        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.part;
         row[k] = sh.by_row(i);
         c[k] = 8 * (i - row[k] * sh.per_row);
-        if (i - k * sh.half >= sh.half || row[k] >= sh.rows) c[k] = sh.O + 8 * sl;  // nothing exists
+        if (i - k * sh.part >= sh.part || row[k] >= sh.rows) c[k] = sh.O + 8 * sl;  // nothing exists
         const int first = c[k] - 8 * sl;
         const T* p = X + int64_t(row[k]) * ldx + first + sl;
 #pragma unroll
         for (int j = 0; j < 8; ++j) t[k][j] = first + j * kL + sl < sh.O ? to_f32(p[j * kL]) : 0.f;
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kQuantizeParts; ++k) {
         float v[8];
         turn_to_groups<kL>(t[k], v, turn + 8 * (threadIdx.x - sl), sl);
         mx_store_block(v, max(0, min(8, sh.O - c[k])), Q.q4, Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]),
@@ -108,20 +110,20 @@ __device__ __forceinline__ void decode8(const uint8_t* q, const uint8_t* s, bool
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(MxView Q, Shape sh, T* __restrict__ Y, int64_t ldy) {
-    float v[2][8];
-    int row[2], c[2];
-    bool live[2];
+    float v[kDequantizeParts][8];
+    int row[kDequantizeParts], c[kDequantizeParts];
+    bool live[kDequantizeParts];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.half;
+    for (int k = 0; k < kDequantizeParts; ++k) {
+        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.part;
         row[k] = sh.by_row(i);
         c[k] = 8 * (i - row[k] * sh.per_row);
-        live[k] = i - k * sh.half < sh.half && row[k] < sh.rows && c[k] < sh.O;
+        live[k] = i - k * sh.part < sh.part && row[k] < sh.rows && c[k] < sh.O;
         if (live[k])
             decode8(Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]), Q.s + int64_t(row[k]) * Q.lds + c[k] / kMxBlock, Q.q4, 8, true, v[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < kDequantizeParts; ++k)
         if (live[k]) store8(Y + int64_t(row[k]) * ldy + c[k], 8, true, v[k]);
 }
 
@@ -129,19 +131,19 @@ template <typename T, int kL>
 __global__ void __launch_bounds__(kThreads) mx_dequantize_columns_kernel(MxView Q, Shape sh, T* __restrict__ Y, int64_t ldy) {
     __shared__ __align__(16) float turn[8 * kThreads];
     const int sl = threadIdx.x % kL;
-    float v[2][8];
-    int row[2], c[2];
+    float v[kDequantizeParts][8];
+    int row[kDequantizeParts], c[kDequantizeParts];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.half;
+    for (int k = 0; k < kDequantizeParts; ++k) {
+        const int i = int(blockIdx.x) * kThreads + int(threadIdx.x) + k * sh.part;
         row[k] = sh.by_row(i);
         c[k] = 8 * (i - row[k] * sh.per_row);
-        if (i - k * sh.half >= sh.half || row[k] >= sh.rows) c[k] = sh.O + 8 * sl;  // nothing exists
+        if (i - k * sh.part >= sh.part || row[k] >= sh.rows) c[k] = sh.O + 8 * sl;  // nothing exists
         decode8(Q.q + int64_t(row[k]) * Q.ldq + (Q.q4 ? c[k] / 2 : c[k]), Q.s + int64_t(row[k]) * Q.lds + c[k] / kMxBlock, Q.q4,
                 max(0, min(8, sh.O - c[k])), sh.vec_q, v[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kDequantizeParts; ++k) {
         float t[8];
         turn_to_columns<kL>(v[k], t, turn + 8 * (threadIdx.x - sl), sl);
         const int first = c[k] - 8 * sl;
@@ -159,18 +161,18 @@ bool rows_aligned(const void* p, int64_t ld_bytes, int64_t bytes) {
 // Calls launch(first row, shape, blocks, lanes) for slices of rows whose work numbers fit 31 bits; lanes = 0: aligned
 // rows, else the kL of the other form.
 template <typename T, class Fn>
-cudaError_t sliced(const DenseView& X, int64_t rows, int O, const MxView& Q, Fn&& launch) {
+cudaError_t sliced(const DenseView& X, int64_t rows, int O, const MxView& Q, int parts, Fn&& launch) {
     const bool vec_q = rows_aligned(Q.q, Q.ldq, Q.q4 ? 4 : 8);
     const bool vec = O % 8 == 0 && rows_aligned(X.p, X.ld * int64_t(sizeof(T)), 16) && vec_q;
     int span = 4;  // groups of eight columns
     if (!vec)
         while (span < 32 && 8 * span < O) span *= 2;
     const int per_row = (O + 8 * span - 1) / (8 * span) * span;
-    const int64_t most = std::max<int64_t>(1, int64_t(0x7ff00000) / per_row);
+    const int64_t most = std::max<int64_t>(1, int64_t(0x7f000000) / per_row);
     for (int64_t r = 0; r < rows; r += most) {
         const int64_t n = std::min(most, rows - r);
-        const int64_t half = (n * per_row / span + 1) / 2 * span;  // whole spans
-        launch(r, Shape{int(n), O, per_row, int(half), Divisor(per_row), vec_q}, unsigned((half + kThreads - 1) / kThreads), vec ? 0 : span);
+        const int64_t part = (n * per_row / span + parts - 1) / parts * span;  // whole spans
+        launch(r, Shape{int(n), O, per_row, int(part), Divisor(per_row), vec_q}, unsigned((part + kThreads - 1) / kThreads), vec ? 0 : span);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
     }
@@ -185,7 +187,7 @@ MxView from_row(MxView Q, int64_t r) {
 
 template <typename T>
 cudaError_t quantize_t(const DenseView& X, int64_t rows, int O, const MxView& Q, cudaStream_t st) {
-    return sliced<T>(X, rows, O, Q, [&](int64_t r, const Shape& sh, unsigned blocks, int lanes) {
+    return sliced<T>(X, rows, O, Q, kQuantizeParts, [&](int64_t r, const Shape& sh, unsigned blocks, int lanes) {
         const T* x = static_cast<const T*>(X.p) + r * X.ld;
         const MxView q = from_row(Q, r);
         if (lanes == 0) mx_quantize_kernel<T><<<blocks, kThreads, 0, st>>>(x, X.ld, sh, q);
@@ -198,7 +200,7 @@ cudaError_t quantize_t(const DenseView& X, int64_t rows, int O, const MxView& Q,
 
 template <typename T>
 cudaError_t dequantize_t(const MxView& Q, int64_t rows, int O, const DenseView& Y, cudaStream_t st) {
-    return sliced<T>(Y, rows, O, Q, [&](int64_t r, const Shape& sh, unsigned blocks, int lanes) {
+    return sliced<T>(Y, rows, O, Q, kDequantizeParts, [&](int64_t r, const Shape& sh, unsigned blocks, int lanes) {
         T* y = static_cast<T*>(Y.p) + r * Y.ld;
         const MxView q = from_row(Q, r);
         if (lanes == 0) mx_dequantize_kernel<T><<<blocks, kThreads, 0, st>>>(q, sh, y, Y.ld);
