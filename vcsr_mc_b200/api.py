@@ -14,6 +14,7 @@ every computation runs in libvcsrmc.so.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from typing import Optional
@@ -335,6 +336,7 @@ def spmm(dV: DeviceVCSRMC, B, C, tileK: int = 128, accumulate: bool = False, str
 
 
 MX_BLOCK = 32  # columns of an MX matrix that share a scale
+_NO_GUARD = contextlib.nullcontext()
 
 
 def _invalid(message: str) -> VcsrmcError:
@@ -383,13 +385,13 @@ class MXDense:
 
     @staticmethod
     def empty(rows: int, cols: int, kind: int = MXF8, device=None) -> "MXDense":
-        """An MXDense to write to. Its rows start at multiples of 16 bytes (8 columns of scales: 4), whatever `cols` is, so that
+        """An MXDense to write to. Its rows start at multiples of 16 bytes (those of its scales: 4), whatever `cols` is, so that
         every operator can use its widest loads and stores."""
-        import torch
-        if kind not in (MXF8, MXF4):
+        torch = _torch or _load_torch()
+        if kind != MXF8 and kind != MXF4:
             raise _invalid("the microscaled kind must be MXF8 or MXF4")
-        width, blocks = (cols if kind == MXF8 else (cols + 1) // 2), -(-cols // MX_BLOCK)
-        ldq, lds = -(-width // 16) * 16, -(-blocks // 4) * 4
+        width, blocks = (cols if kind == MXF8 else (cols + 1) // 2), (cols + MX_BLOCK - 1) // MX_BLOCK
+        ldq, lds = (width + 15) & -16, (blocks + 3) & -4
         data = torch.empty(rows, ldq, dtype=torch.float8_e4m3fn if kind == MXF8 else torch.uint8, device=device)
         scale = torch.empty(rows, lds, dtype=torch.float8_e8m0fnu, device=device)
         if ldq != width:
@@ -406,72 +408,73 @@ def _row_stride(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
-_DENSE = None  # torch dtype -> VCSRMC code
+_torch = None
+_DENSE = {}  # torch dtype -> VCSRMC code
 
 
-def _dense_dtype(t, what: str) -> int:
-    global _DENSE
-    if _DENSE is None:
-        import torch
-        _DENSE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    code = _DENSE.get(getattr(t, "dtype", None))
-    if code is None:
-        raise _invalid(f"{what} must be a float32, float16 or bfloat16 tensor")
-    return code
+def _load_torch():
+    """torch, imported at the first microscaled call."""
+    global _torch
+    import torch
+    _DENSE.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    torch.cuda.is_available() and torch.cuda.init()
+    _torch = torch
+    return torch
 
 
-def _dense_2d(t, what: str, device=None, shape=None, dtype=None):
-    """Checks a dense matrix and returns (pointer, row stride)."""
-    shp = getattr(t, "shape", ())
-    if len(shp) != 2 or not t.is_cuda:
-        raise _invalid(f"{what} must be a 2-D CUDA tensor")
-    ld, step = t.stride()
-    if step != 1 and shp[1] > 1:
+def _dense(t, what: str):
+    """(pointer, row stride, dtype code, rows, columns, device index) of a dense matrix that an operator takes."""
+    try:
+        rows, cols = t.shape
+        ld, step = t.stride()
+        device = t.get_device()
+        code = _DENSE[t.dtype]
+    except (AttributeError, ValueError, KeyError, TypeError):
+        raise _invalid(f"{what} must be a 2-D float32, float16 or bfloat16 tensor") from None
+    if device < 0:
+        raise _invalid(f"{what} must be a CUDA tensor")
+    if step != 1 and cols > 1:
         raise _invalid(f"the columns of {what} must be contiguous")
-    if shp[0] <= 1:
-        ld = max(shp[1], 1)
-    elif ld < shp[1]:
+    if rows <= 1:
+        ld = cols or 1  # torch leaves the stride of a single row open
+    elif ld < cols:
         raise _invalid(f"the rows of {what} must not overlap")
-    if device is not None and t.device != device:
-        raise _invalid(f"{what} must be on {device}, with the other tensors")
-    if shape is not None and shp != shape:
-        raise _invalid(f"{what} must be {tuple(shape)}, got {tuple(shp)}")
-    if dtype is not None and t.dtype != dtype:
-        raise _invalid(f"{what} must be {dtype}, got {t.dtype}")
-    return t.data_ptr(), ld
+    return t.data_ptr(), ld, code, rows, cols, device
 
 
-def _vector(t, what: str, device, n: int, dtype=None) -> int:
-    """Checks a contiguous vector of n values and returns its pointer."""
-    if len(getattr(t, "shape", ())) != 1 or t.shape[0] != n or t.device != device or (n > 1 and t.stride(0) != 1):
-        raise _invalid(f"{what} must be a contiguous tensor of {n} values on {device}")
-    if dtype is not None and t.dtype != dtype:
-        raise _invalid(f"{what} must be {dtype}, got {t.dtype}")
-    return t.data_ptr()
+def _like(t, what: str, rows: int, cols: int, device: int, code: Optional[int] = None):
+    """(pointer, row stride, dtype code) of a matrix that goes with another one: its shape and device, and a type if one is given."""
+    p, ld, c, r, n, d = _dense(t, what)
+    if r != rows or n != cols or d != device:
+        raise _invalid(f"{what} must be {rows} x {cols} on cuda:{device}, with the other tensors")
+    if code is not None and c != code:
+        raise _invalid(f"{what} has another type than the tensors it goes with")
+    return p, ld, c
 
 
-def _on(device, stream):
+def _vector(t, what: str, device: int, n: int):
+    """(pointer, dtype code) of a contiguous vector of n values."""
+    try:
+        (m,), (step,) = t.shape, t.stride()
+        if m == n and t.get_device() == device and (step == 1 or n <= 1):
+            return t.data_ptr(), _DENSE[t.dtype]
+    except (AttributeError, ValueError, KeyError, TypeError):
+        pass
+    raise _invalid(f"{what} must be a contiguous float32, float16 or bfloat16 tensor of {n} values on cuda:{device}")
+
+
+def _on(torch, device: int, stream):
     """(guard, stream handle): the guard makes `device` and `stream` (None: torch's current one there) current, so that what is
     allocated under it belongs to the stream that uses it; it is None where they are current already."""
-    import torch
-    if device.type != "cuda":
-        raise _invalid("microscaled operators run on CUDA tensors")
     if stream is None:
-        guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
-        return guard, torch._C._cuda_getCurrentRawStream(device.index)
+        guard = torch.cuda.device(device) if torch._C._cuda_getDevice() != device else None
+        return guard, torch._C._cuda_getCurrentRawStream(device)
     if not isinstance(stream, torch.cuda.Stream):
         raw = int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
         stream = torch.cuda.ExternalStream(raw, device=device)
-    if stream.device != device:
-        raise _invalid(f"the stream must be on {device}, with the tensors")
+    if stream.device.index != device:
+        raise _invalid(f"the stream must be on cuda:{device}, with the tensors")
     return torch.cuda.stream(stream), stream.cuda_stream
-
-
-def _under(guard, fn):
-    if guard is None:
-        return fn()
-    with guard:
-        return fn()
 
 
 def _out_mx(out: Optional[MXDense], rows: int, cols: int, kind: int, device) -> MXDense:
@@ -483,57 +486,53 @@ def _out_mx(out: Optional[MXDense], rows: int, cols: int, kind: int, device) -> 
 
 
 def _spmm_mx(dV: DeviceVCSRMC, B: MXDense, C, tileK: int, accumulate: bool, stream, O: Optional[int], plan: int):
-    import torch
+    torch = _torch or _load_torch()
+    c, ldc, c_dtype, rows, cols, device = _dense(C, "C")
     O = B.cols if O is None else O
-    c, ldc = _dense_2d(C, "C", B.device, None, torch.float32)
-    if C.device.index != dV.device:
+    if c_dtype != F32:
+        raise _invalid("C must be float32")
+    if device != dV.device or B.device.type != "cuda" or B.device.index != device:
         raise _invalid("A, B and C must be on the same device")
-    if plan not in (PLAN_AUTO, PLAN_ROWS):
+    if plan != PLAN_AUTO and plan != PLAN_ROWS:
         raise _invalid("a microscaled B runs on the ROWS plan")
     if tileK not in (16, 32, 64, 128, 256):
         raise _invalid("tileK must be one of 16, 32, 64, 128, 256")
-    if B.cols < O or C.shape[1] < O or B.rows < dV.N or C.shape[0] < dV.M:
+    if B.cols < O or cols < O or B.rows < dV.N or rows < dV.M:
         raise _invalid("B and C must hold A's columns and rows, with >= O columns")
-    guard, st = _on(C.device, stream)
+    guard, st = _on(torch, device, stream)
     n = dV.mx_workspace(O)
-
-    def run():
+    with guard or _NO_GUARD:
         ws = torch.empty(n, dtype=torch.uint8, device=C.device) if n else None
-        call("vcsrmc_spmm_mx", dV.handle, *B._args, O, c, ldc, 1 if accumulate else 0, None if ws is None else ws.data_ptr(), n, st)
-
-    _under(guard, run)
+        call("vcsrmc_spmm_mx", dV.handle, *B._args, O, c, ldc, 1 if accumulate else 0, ws.data_ptr() if n else None, n, st)
     return C
 
 
 def mx_quantize(X, kind: int = MXF8, out: Optional[MXDense] = None, stream=None) -> MXDense:
     """X (float32, float16 or bfloat16) in 8 (MXF8) or 4 bits (MXF4): the scale of 32 columns is the smallest power of two
     under which their largest magnitude fits the element type; elements are rounded to nearest, ties to even."""
-    x, ldx = _dense_2d(X, "X")
-    x_dtype = _dense_dtype(X, "X")
-    rows, cols = X.shape
-    guard, st = _on(X.device, stream)
-
-    def run():
+    torch = _torch or _load_torch()
+    x, ldx, x_dtype, rows, cols, device = _dense(X, "X")
+    guard, st = _on(torch, device, stream)
+    with guard or _NO_GUARD:
         Q = _out_mx(out, rows, cols, kind, X.device)
         q, q_dtype, ldq, s, lds = Q._args
         call("vcsrmc_mx_quantize", x, x_dtype, ldx, rows, cols, q_dtype, q, ldq, s, lds, st)
-        return Q
-
-    return _under(guard, run)
+    return Q
 
 
 def mx_dequantize(Q: MXDense, dtype=None, out=None, stream=None):
     """The values an MXDense stands for, rounded to `dtype` (default float32)."""
-    import torch
-    guard, st = _on(Q.device, stream)
-
-    def run():
+    torch = _torch or _load_torch()
+    if Q.device.type != "cuda":
+        raise _invalid("Q must be on a CUDA device")
+    guard, st = _on(torch, Q.device.index, stream)
+    with guard or _NO_GUARD:
         Y = torch.empty(Q.rows, Q.cols, dtype=dtype or torch.float32, device=Q.device) if out is None else out
-        y, ldy = _dense_2d(Y, "out", Q.device, Q.shape, dtype)
-        call("vcsrmc_mx_dequantize", *Q._args, Q.rows, Q.cols, y, _dense_dtype(Y, "out"), ldy, st)
-        return Y
-
-    return _under(guard, run)
+        if dtype is not None and Y.dtype != dtype:
+            raise _invalid(f"out must be {dtype}, got {Y.dtype}")
+        y, ldy, y_dtype = _like(Y, "out", Q.rows, Q.cols, Q.device.index)
+        call("vcsrmc_mx_dequantize", *Q._args, Q.rows, Q.cols, y, y_dtype, ldy, st)
+    return Y
 
 
 def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, out: Optional[MXDense] = None, residual_out=None,
@@ -541,63 +540,53 @@ def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, 
     """(Q, residual_out, inv_rms): s = X + residual, rounded to the residual's type (residual_out); inv_rms = 1 / sqrt(mean(s^2) +
     eps) of every row (float32); Q = MX(s * inv_rms * weight). The residual has X's type, or X is float32 (a product's C). Without a
     residual s is X, which is then returned in residual_out's place. residual_out may be the residual, or X of the same type (in place)."""
-    import torch
-    x, ldx = _dense_2d(X, "X")
-    x_dtype, device, shape = _dense_dtype(X, "X"), X.device, X.shape
-    rows, cols = shape
-    w, w_dtype = _vector(weight, "weight", device, cols), _dense_dtype(weight, "weight")
-    if residual is None:
-        r, ldr, r_type, r_dtype = None, 0, X.dtype, x_dtype
-    else:
-        r, ldr = _dense_2d(residual, "residual", device, shape)
-        r_type, r_dtype = residual.dtype, _dense_dtype(residual, "residual")
-    guard, st = _on(device, stream)
-
-    def run():
-        h = residual_out
-        if h is not None:
-            o, ldo = _dense_2d(h, "residual_out", device, shape, r_type)
+    torch = _torch or _load_torch()
+    x, ldx, x_dtype, rows, cols, device = _dense(X, "X")
+    w, w_dtype = _vector(weight, "weight", device, cols)
+    r, ldr, r_dtype = (None, 0, x_dtype) if residual is None else _like(residual, "residual", rows, cols, device)
+    at = X.device
+    guard, st = _on(torch, device, stream)
+    with guard or _NO_GUARD:
+        o, ldo = None, 0
+        if residual_out is not None:
+            o, ldo, _ = _like(residual_out, "residual_out", rows, cols, device, r_dtype)
         elif residual is not None:
-            h = torch.empty(rows, cols, dtype=r_type, device=device)
-            o, ldo = h.data_ptr(), max(cols, 1)
-        else:
-            o, ldo = None, 0
-        Q = _out_mx(out, rows, cols, kind, device)
-        inv_rms = torch.empty(rows, dtype=torch.float32, device=device)
+            residual_out = torch.empty(rows, cols, dtype=residual.dtype, device=at)
+            o, ldo = residual_out.data_ptr(), cols
+        Q = _out_mx(out, rows, cols, kind, at)
+        inv_rms = torch.empty(rows, dtype=torch.float32, device=at)
         q, q_dtype, ldq, s, lds = Q._args
         call("vcsrmc_add_rms_norm", x, x_dtype, ldx, r, ldr, o, ldo, r_dtype, w, w_dtype, eps, rows, cols, q_dtype, q, ldq, s, lds,
              inv_rms.data_ptr(), st)
-        return Q, X if h is None else h, inv_rms
-
-    return _under(guard, run)
+    return Q, X if residual_out is None else residual_out, inv_rms
 
 
 def add_rms_norm_backward(dY, weight, hidden, inv_rms, d_residual=None, out=None, stream=None):
     """(dX, dweight) of add_rms_norm: dY is the gradient of the values Q stands for (float32 or hidden's type; the elements' rounding
     counts as the identity), hidden and inv_rms are what the forward call returned, d_residual the gradient of its residual_out. dX, in
     hidden's type, is the gradient of X and of the residual; dweight is float32. out (dX) may be d_residual, or dY of the same type."""
-    import torch
-    dy, lddy = _dense_2d(dY, "dY")
-    dy_dtype, device, shape = _dense_dtype(dY, "dY"), dY.device, dY.shape
-    rows, cols = shape
-    w, w_dtype = _vector(weight, "weight", device, cols), _dense_dtype(weight, "weight")
-    h, ldh = _dense_2d(hidden, "hidden", device, shape)
-    r_dtype = _dense_dtype(hidden, "hidden")
-    inv = _vector(inv_rms, "inv_rms", device, rows, torch.float32)
-    dr, lddr = (None, 0) if d_residual is None else _dense_2d(d_residual, "d_residual", device, shape, hidden.dtype)
-    guard, st = _on(device, stream)
-
-    def run():
-        dX = torch.empty(rows, cols, dtype=hidden.dtype, device=device) if out is None else out
-        dx, lddx = _dense_2d(dX, "out", device, shape, hidden.dtype)
-        dweight = torch.empty(cols, dtype=torch.float32, device=device)
-        n = _grad_workspace(rows, cols, device.index)
-        ws = torch.empty(n, dtype=torch.uint8, device=device)
+    torch = _torch or _load_torch()
+    dy, lddy, dy_dtype, rows, cols, device = _dense(dY, "dY")
+    w, w_dtype = _vector(weight, "weight", device, cols)
+    h, ldh, r_dtype = _like(hidden, "hidden", rows, cols, device)
+    inv, inv_dtype = _vector(inv_rms, "inv_rms", device, rows)
+    if inv_dtype != F32:
+        raise _invalid("inv_rms must be float32")
+    dr, lddr, _ = (None, 0, 0) if d_residual is None else _like(d_residual, "d_residual", rows, cols, device, r_dtype)
+    at = dY.device
+    guard, st = _on(torch, device, stream)
+    with guard or _NO_GUARD:
+        if out is None:
+            out = torch.empty(rows, cols, dtype=hidden.dtype, device=at)
+            dx, lddx = out.data_ptr(), cols
+        else:
+            dx, lddx, _ = _like(out, "out", rows, cols, device, r_dtype)
+        dweight = torch.empty(cols, dtype=torch.float32, device=at)
+        n = _grad_workspace(rows, cols, device)
+        ws = torch.empty(n, dtype=torch.uint8, device=at)
         call("vcsrmc_add_rms_norm_backward", dy, dy_dtype, lddy, dr, lddr, h, ldh, r_dtype, w, w_dtype, inv, rows, cols, dx, lddx,
              dweight.data_ptr(), ws.data_ptr(), n, st)
-        return dX, dweight
-
-    return _under(guard, run)
+    return out, dweight
 
 
 @functools.lru_cache(maxsize=256)
