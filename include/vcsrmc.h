@@ -277,9 +277,10 @@ int vcsrmc_mx_dequantize(const void* Q, int q_dtype, int64_t ldq, const uint8_t*
                          int64_t rows, int32_t O, void* Y, int y_dtype, int64_t ldy, void* stream);
 /* C[M x O] (+)= A * B with an MX operand B (N rows): both formats, ROWS layout, fp32 sums whose order
  * is fixed (the same call gives the same bits). |a| * 2^(code - 127) of an entry and a block must be
- * finite. The workspace (vcsrmc_spmm_mx_workspace bytes, 0 for a matrix without split rows; 16-byte
- * aligned) is the caller's, so products of one handle may be in flight on several streams or in several
- * graphs as long as each has its own; it need not be initialised. */
+ * finite, and counts as zero below fp32's normal range (2^-126), as in blocks of code 0. The workspace
+ * (vcsrmc_spmm_mx_workspace bytes, 0 for a matrix without rows to split; 16-byte aligned) is the caller's,
+ * so products of one handle may be in flight on several streams or in several graphs as long as each has
+ * its own; it need not be initialised. */
 int vcsrmc_spmm_mx_workspace(const vcsrmc_device_format* d, int32_t O, int64_t* bytes);
 int vcsrmc_spmm_mx(const vcsrmc_device_format* d, const void* Q, int q_dtype, int64_t ldq,
                    const uint8_t* S, int64_t lds, int32_t O, float* C, int64_t ldc, int accumulate,

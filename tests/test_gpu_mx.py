@@ -270,6 +270,60 @@ def test_product_scaled_format_hot_columns_and_extremes(cuda):
     check_product(dV, csr, codes, scales, "mxf8")
 
 
+def test_product_ends_of_the_scale_range(cuda):
+    """Code 0 and subnormal products count as zero, code 254 as what it says; in the FP16 and the FP32 format."""
+    M, N, O = 33, 40, 96
+    csr = sparse(M, N, 0.4, 9)
+    codes, scales = features(N, O, 10, "mxf8")
+    scales[:, 0], scales[::2, 1], scales[1::2, 1], scales[:, 2] = 0, 0, 127, 254
+    codes[:, 64:] &= 0x87  # subnormal elements, so that the sums stay finite
+    known = scales.copy()
+    known[known == 0] = 127
+    zeroed = codes.copy()
+    zeroed[np.repeat(scales == 0, 32, 1)] = 0
+    want, size, n = ref.product(*csr, ref.values(zeroed, known, "mxf8"))
+    for fp32 in (False, True):
+        dV = handle(M, N, *csr, fp32)
+        C = torch.empty(M, O, device="cuda")
+        vm.spmm(dV, to_mx(codes, scales, "mxf8"), C)
+        assert np.all(np.abs(np64(C) - want) <= (n + 4) * U * size)
+
+
+@pytest.mark.parametrize("M,N", [(0, 7), (7, 0), (1, 1)])
+def test_product_empty_matrices(cuda, M, N):
+    rp, none = np.zeros(M + 1, np.int32), np.zeros(0)
+    dV = handle(M, N, rp, none.astype(np.int32), none.astype(np.float32), False)
+    Q = vm.mx_quantize(torch.ones(N, 33, device="cuda"), vm.MXF4)
+    C = torch.full((M, 33), 5.0, device="cuda")
+    vm.spmm(dV, Q, C, accumulate=True)
+    assert bool((C == 5).all())
+    vm.spmm(dV, Q, C)
+    assert bool((C == 0).all())
+
+
+def test_product_far_offsets(cuda):
+    """An operand and a result past 4 GiB, and scales past 2^31 bytes into their array's rows."""
+    N, M, O = 34_000_000, 9_000_000, 130  # elements of 144-byte rows: 4.9 GB; C 4.7 GB
+    data = torch.zeros(N, 144, dtype=torch.uint8, device="cuda")
+    scale = torch.full((N, 64), 127, dtype=torch.uint8, device="cuda")
+    cols = torch.tensor([0, 7, N // 2 + 1, N - 2, N - 1], device="cuda")
+    codes, scales = features(5, O, 3, "mxf8")
+    data[cols, :O] = torch.from_numpy(codes).cuda()
+    scale[cols, 57:62] = torch.from_numpy(scales).cuda()
+    Q = vm.MXDense(data[:, :O].view(torch.float8_e4m3fn), scale[:, 57:62], cols=O)
+    rp = torch.zeros(M + 1, dtype=torch.int32, device="cuda")
+    rp[1:] = 2
+    rp[M:] = 5
+    dV = vm.build_vcsr_mc_device(rp, cols[torch.tensor([0, 3, 1, 2, 4], device="cuda")].int(), torch.tensor([1.0, 2, 0.5, -1, 4], device="cuda"), M, N,
+                                 segw=32, plans=[vm.PLAN_ROWS])
+    C = torch.full((M, O), 9.0, device="cuda")
+    vm.spmm(dV, Q, C)
+    B = ref.values(codes, scales, "mxf8")
+    for row, want in ((0, B[0] + 2 * B[3]), (M - 1, 0.5 * B[1] - B[2] + 4 * B[4])):
+        assert np.all(np.abs(np64(C[row]) - want) <= 7 * U * np.abs(4 * B).sum(0))
+    assert not bool(C[1:M - 1].any())
+
+
 def test_product_refusals(cuda):
     M, N = 20, 130
     csr = sparse(M, N, 0.3, 5, long_row=1)
@@ -284,7 +338,7 @@ def test_product_refusals(cuda):
             call()
     from vcsr_mc_b200 import _lib
     with pytest.raises(vm.VcsrmcError):  # no workspace for the split row
-        _lib.call("vcsrmc_spmm_mx", dV.handle, *Q._args, 64, C.data_ptr(), 64, 0, None, 0, None)
+        _lib.call("vcsrmc_spmm_mx", dV.handle, *Q._args(), 64, C.data_ptr(), 64, 0, None, 0, None)
     only_segment = vm.upload_vcsr_mc_device(vm.csr_to_vcsr_mc(vm.CSR.from_arrays(M, N, *csr), segw=32), plans=[vm.PLAN_SEGMENT])
     with pytest.raises(vm.VcsrmcError):
         vm.spmm(only_segment, Q, C)
@@ -421,6 +475,24 @@ def test_norm_backward_against_differences(cuda):
         assert abs((loss(x, wd + d) - loss(x, wd - d)) / (2 * step) - float(dw[j])) < 1e-4
 
 
+def test_products_in_flight_together(cuda):
+    """One handle on two streams at once, rows split into chunks: each product has its own workspace."""
+    M, N, O = 40, 4000, 128
+    csr = sparse(M, N, 0.5, 11)
+    dV = handle(M, N, *csr, False, rows_unit_nnz=16)
+    Qs = [to_mx(*features(N, O, 20 + i, "mxf4"), "mxf4") for i in range(2)]
+    alone = [vm.spmm(dV, Q, torch.empty(M, O, device="cuda")) for Q in Qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = [[torch.empty(M, O, device="cuda") for _ in range(20)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for k in range(20):
+        for i in range(2):
+            vm.spmm(dV, Qs[i], results[i][k], stream=streams[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(C, alone[i]) for i in range(2) for C in results[i])
+
+
 # ---- together ----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", KINDS)
 def test_layers_run_captured_and_on_streams(cuda, kind):
@@ -441,6 +513,7 @@ def test_layers_run_captured_and_on_streams(cuda, kind):
         return C, h, inv
 
     eager = layers(X0)
+    eager += vm.add_rms_norm_backward(eager[0], w, eager[1], eager[2], d_residual=eager[1])
     # layer by layer against the definitions, from the library's own inputs of each step
     Q = vm.mx_quantize(X0, KINDS[kind])
     C = check_product(dV, (rp, col, val), *codes_of(Q), kind)
@@ -453,14 +526,17 @@ def test_layers_run_captured_and_on_streams(cuda, kind):
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            layers(X)
+            warm = layers(X)
+            vm.add_rms_norm_backward(warm[0], w, warm[1], warm[2], d_residual=warm[1])
         torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = layers(X)
+            out += vm.add_rms_norm_backward(out[0], w, out[1], out[2], d_residual=out[1])
         graphs.append((graph, X, out))
     graphs[1][1].copy_(X0 * 2)
     two = layers(X0 * 2)
+    two += vm.add_rms_norm_backward(two[0], w, two[1], two[2], d_residual=two[1])
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
     torch.cuda.synchronize()
     for _ in range(3):

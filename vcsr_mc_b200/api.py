@@ -351,7 +351,7 @@ class MXDense:
     scale: float8_e8m0fnu (or uint8) [rows, ceil(cols / 32)]
     Rows may be strided; columns may not. `cols` is needed for an odd number of MXF4 columns."""
 
-    __slots__ = ("data", "scale", "kind", "rows", "cols", "device", "_args")
+    __slots__ = ("data", "scale", "kind", "rows", "cols", "device", "_ldq", "_lds")
 
     def __init__(self, data, scale, cols: Optional[int] = None):
         import torch
@@ -376,8 +376,11 @@ class MXDense:
 
     def _set(self, data, scale, kind, rows, cols, device, ldq, lds):
         self.data, self.scale, self.kind, self.rows, self.cols, self.device = data, scale, kind, rows, cols, device
-        # pointer, type, row stride, scale pointer and scale row stride, as the C ABI takes them
-        self._args = (data.data_ptr(), kind, ldq, scale.data_ptr(), lds)
+        self._ldq, self._lds = ldq, lds
+
+    def _args(self):
+        """Pointer, type, row stride, scale pointer and scale row stride, as the C ABI takes them."""
+        return self.data.data_ptr(), self.kind, self._ldq, self.scale.data_ptr(), self._lds
 
     @property
     def shape(self):
@@ -503,7 +506,7 @@ def _spmm_mx(dV: DeviceVCSRMC, B: MXDense, C, tileK: int, accumulate: bool, stre
     n = dV.mx_workspace(O)
     with guard or _NO_GUARD:
         ws = torch.empty(n, dtype=torch.uint8, device=C.device) if n else None
-        call("vcsrmc_spmm_mx", dV.handle, *B._args, O, c, ldc, 1 if accumulate else 0, ws.data_ptr() if n else None, n, st)
+        call("vcsrmc_spmm_mx", dV.handle, *B._args(), O, c, ldc, 1 if accumulate else 0, ws.data_ptr() if n else None, n, st)
     return C
 
 
@@ -515,7 +518,7 @@ def mx_quantize(X, kind: int = MXF8, out: Optional[MXDense] = None, stream=None)
     guard, st = _on(torch, device, stream)
     with guard or _NO_GUARD:
         Q = _out_mx(out, rows, cols, kind, X.device)
-        q, q_dtype, ldq, s, lds = Q._args
+        q, q_dtype, ldq, s, lds = Q._args()
         call("vcsrmc_mx_quantize", x, x_dtype, ldx, rows, cols, q_dtype, q, ldq, s, lds, st)
     return Q
 
@@ -531,7 +534,7 @@ def mx_dequantize(Q: MXDense, dtype=None, out=None, stream=None):
         if dtype is not None and Y.dtype != dtype:
             raise _invalid(f"out must be {dtype}, got {Y.dtype}")
         y, ldy, y_dtype = _like(Y, "out", Q.rows, Q.cols, Q.device.index)
-        call("vcsrmc_mx_dequantize", *Q._args, Q.rows, Q.cols, y, y_dtype, ldy, st)
+        call("vcsrmc_mx_dequantize", *Q._args(), Q.rows, Q.cols, y, y_dtype, ldy, st)
     return Y
 
 
@@ -555,7 +558,7 @@ def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, 
             o, ldo = residual_out.data_ptr(), cols
         Q = _out_mx(out, rows, cols, kind, at)
         inv_rms = torch.empty(rows, dtype=torch.float32, device=at)
-        q, q_dtype, ldq, s, lds = Q._args
+        q, q_dtype, ldq, s, lds = Q._args()
         call("vcsrmc_add_rms_norm", x, x_dtype, ldx, r, ldr, o, ldo, r_dtype, w, w_dtype, eps, rows, cols, q_dtype, q, ldq, s, lds,
              inv_rms.data_ptr(), st)
     return Q, X if residual_out is None else residual_out, inv_rms
