@@ -565,3 +565,21 @@ def test_layers_run_captured_and_on_streams(cuda, kind):
     dB = check_product(dT, (rpt, rows, val[order]), *codes_of(dC), kind)
     dx, dw = vm.add_rms_norm_backward(dB, w, eager[1], eager[2])
     assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dw).all())
+
+
+@pytest.mark.parametrize("O", [24, 33, 128])
+def test_driver_microscaled(cuda, O):
+    """spmm_vcsr's microscaled algorithms pass its own check against the fp64 product with the values that B then stands for."""
+    import csv
+    import io
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([os.path.join(root, "vcsr_mc_b200", "spmm_vcsr"), "--gen", "c1", "--O", str(O), "--algo", "vcsr_mc,vcsr_mc_mxf8,vcsr_mc_mxf4",
+                          "--bdist", "normal", "--repeat", "2", "--warmup", "1", "--csv"], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr
+    rows = {r["algo"]: r for r in csv.DictReader(io.StringIO(out.stdout))}
+    assert set(rows) == {"vcsr_mc", "vcsr_mc_mxf8", "vcsr_mc_mxf4"}
+    assert all(r["validation"] == "pass" and float(r["gbps_alg"]) > 0 for r in rows.values())
+    # fp16 values of A are all that is rounded: half a step of 2^-11 at most, and the check's bound of 3e-3 is far
+    assert all(float(rows[k]["rel_l2"]) <= 2.0 ** -11 for k in ("vcsr_mc_mxf8", "vcsr_mc_mxf4"))

@@ -61,7 +61,9 @@ void usage() {
     std::printf(
         "Usage: spmm_vcsr (--mtx file.mtx | --gen c1|c2|c3|c3links|rmat[:scale]) --O 128 [options]\n"
         "Algorithms: vcsr_mc (FP16 A/B, FP32 accumulate), vcsr_mc_fp32, cusparse (FP32),\n"
-        "            cusparse_fp16 (FP16 A and B, FP32 compute and C), all\n"
+        "            cusparse_fp16 (FP16 A and B, FP32 compute and C), all (those four);\n"
+        "            vcsr_mc_mxf8, vcsr_mc_mxf4 (FP16 A, B microscaled to 8 or 4 bits, checked against the\n"
+        "            product with the values it then stands for)\n"
         "Options: --segw 16 --tileK 64 --repeat 10 --warmup 3 --stat mean|median\n"
         "         --reorder none|rcm --check cpu|none --csv --bdist pattern|normal|uniform|wide\n"
         "         --lenient --seed 0 --plan auto|rows|segment|band|hybrid --b16 --flush-l2 --peak-gbs G\n"
@@ -156,7 +158,7 @@ struct Acceptance {
     double norm_factor, rel_cap;
 };
 Acceptance acceptance_for(const std::string& kernel) {
-    const bool fp16_inputs = kernel == "vcsr_mc" || kernel == "cusparse_fp16";
+    const bool fp16_inputs = kernel == "vcsr_mc" || kernel == "cusparse_fp16" || kernel == "vcsr_mc_mxf8" || kernel == "vcsr_mc_mxf4";
     return fp16_inputs ? Acceptance{3e-3, 1e-1} : Acceptance{1e-4, 1e-2};
 }
 bool accepted(const Fp64Comparison& c, const Acceptance& a, size_t numel) {
@@ -213,7 +215,7 @@ void print_result(const ResultRow& r, const RunColumns& run, bool csv) {
 
 // Compulsory bytes of one SpMM: per entry its column index and value (a_bytes), row_ptr, the
 // `distinct` rows of B that A touches (O values of b_bytes each), and C (fp32) written once.
-double algorithmic_bytes(const CSR& csr, int64_t distinct, int O, int a_bytes, int b_bytes) {
+double algorithmic_bytes(const CSR& csr, int64_t distinct, int O, int a_bytes, double b_bytes) {
     return double(csr.nnz) * (4 + a_bytes) + (double(csr.M) + 1) * 4 + double(distinct) * O * b_bytes +
            double(csr.M) * O * 4;
 }
@@ -276,7 +278,8 @@ static int benchmark_main(int argc, char** argv) {
             default: usage(); return 2;
         }
     }
-    const std::vector<std::string> algorithms = {"all", "vcsr_mc", "vcsr_mc_fp32", "cusparse", "cusparse_fp16"};
+    const std::vector<std::string> algorithms = {"all",      "vcsr_mc",       "vcsr_mc_fp32", "cusparse",
+                                                 "cusparse_fp16", "vcsr_mc_mxf8", "vcsr_mc_mxf4"};
     std::vector<std::string> requested;
     for (size_t pos = 0;;) {
         const size_t comma = algo.find(',', pos);
@@ -287,10 +290,8 @@ static int benchmark_main(int argc, char** argv) {
         if (comma == std::string::npos) break;
         pos = comma + 1;
     }
-    auto selected = [&](const char* name) {
-        return std::find(requested.begin(), requested.end(), "all") != requested.end() ||
-               std::find(requested.begin(), requested.end(), name) != requested.end();
-    };
+    auto named = [&](const char* name) { return std::find(requested.begin(), requested.end(), name) != requested.end(); };
+    auto selected = [&](const char* name) { return named("all") || named(name); };
     if (check != "cpu" && check != "none") throw std::runtime_error("Unknown reference: " + check);
     if ((mtx.empty() == gen.empty()) || optind != argc) { usage(); return 2; }
     if (reorder != "none" && reorder != "rcm") throw std::runtime_error("Unknown reordering: " + reorder);
@@ -412,9 +413,12 @@ static int benchmark_main(int argc, char** argv) {
         row.gflops = row.ms > 0 ? (2.0 * csr.nnz * O) / (row.ms * 1e6) : 0;
         {
             const std::string k(name);
-            const bool fp16_a = k == "vcsr_mc" || k == "cusparse_fp16";
+            const bool mxf8 = k == "vcsr_mc_mxf8", mxf4 = k == "vcsr_mc_mxf4";
+            const bool fp16_a = k == "vcsr_mc" || k == "cusparse_fp16" || mxf8 || mxf4;
             const bool fp16_b = k == "cusparse_fp16" || (k == "vcsr_mc" && b16);
-            const double bytes = algorithmic_bytes(csr, distinct, O, fp16_a ? 2 : 4, fp16_b ? 2 : 4);
+            // a microscaled element and its share of the scale
+            const double b_bytes = mxf8 ? 1 + 1. / 32 : mxf4 ? 0.5 + 1. / 32 : fp16_b ? 2 : 4;
+            const double bytes = algorithmic_bytes(csr, distinct, O, fp16_a ? 2 : 4, b_bytes);
             row.gbps_alg = row.ms > 0 ? bytes / (row.ms * 1e6) : 0;
             if (peak_gbs > 0) row.roofline_frac = row.gbps_alg / peak_gbs;
         }
@@ -510,6 +514,60 @@ static int benchmark_main(int argc, char** argv) {
                 throw std::runtime_error(std::string("cuSPARSE: ") + vcsrmc_cusparse_last_error());
             return ms;
         }, 0.f, 0.f, 0.f, "-");
+    }
+    // last: their check replaces the reference result
+    for (const bool q4 : {false, true}) {
+        const char* name = q4 ? "vcsr_mc_mxf4" : "vcsr_mc_mxf8";
+        if (!named(name)) continue;
+        const int q_dtype = q4 ? VCSRMC_MXF4 : VCSRMC_MXF8;
+        // rows of elements and scales at multiples of 16 and 4 bytes, for the widest loads
+        const int64_t ldq = ((q4 ? (int64_t(O) + 1) / 2 : O) + 15) / 16 * 16, lds = ((int64_t(O) + 31) / 32 + 3) / 4 * 4;
+        uint8_t *dQ = nullptr, *dS = nullptr;
+        void* dW = nullptr;
+        cuda_ok(cudaMalloc(&dQ, size_t(std::max(csr.N, 1)) * ldq), "cudaMalloc");
+        cuda_ok(cudaMalloc(&dS, size_t(std::max(csr.N, 1)) * lds), "cudaMalloc");
+        abi_ok(vcsrmc_mx_quantize(dB, VCSRMC_F32, O, csr.N, O, q_dtype, dQ, ldq, dS, lds, st));
+        if (check == "cpu") {
+            float* dV = nullptr;
+            std::vector<float> hV(elementsB);
+            cuda_ok(cudaMalloc(&dV, std::max<size_t>(elementsB, 1) * sizeof(float)), "cudaMalloc");
+            abi_ok(vcsrmc_mx_dequantize(dQ, q_dtype, ldq, dS, lds, csr.N, O, dV, VCSRMC_F32, O, st));
+            cuda_ok(cudaStreamSynchronize(st), "cudaStreamSynchronize");
+            cuda_ok(cudaMemcpy(hV.data(), dV, elementsB * sizeof(float), cudaMemcpyDeviceToHost), "cudaMemcpy");
+            cudaFree(dV);
+            reference = cpu_reference(csr, hV, O);
+        }
+        vcsrmc_csr* hc = nullptr;
+        vcsrmc_format* hf = nullptr;
+        vcsrmc_device_format* hd = nullptr;
+        abi_ok(vcsrmc_csr_from_arrays(csr.M, csr.N, csr.nnz, csr.row_ptr.data(), csr.col.data(), csr.val.data(), &hc));
+        const float convert = host_ms([&] { abi_ok(vcsrmc_build_host(hc, 0, segw, 0, &hf)); });
+        const float upload = host_ms([&] { abi_ok(vcsrmc_upload_ex(hf, device_id, 1 << VCSRMC_PLAN_ROWS, st, &hd)); });
+        int64_t need = 0;
+        abi_ok(vcsrmc_spmm_mx_workspace(hd, O, &need));
+        if (need > 0) cuda_ok(cudaMalloc(&dW, size_t(need)), "cudaMalloc");
+        measure(name,
+                [&] {
+                    cudaEvent_t a, b;
+                    cudaEventCreate(&a);
+                    cudaEventCreate(&b);
+                    cudaEventRecord(a, st);
+                    abi_ok(vcsrmc_spmm_mx(hd, dQ, q_dtype, ldq, dS, lds, O, dC, O, 1, dW, need, st));
+                    cudaEventRecord(b, st);
+                    cudaEventSynchronize(b);
+                    float ms = 0;
+                    cudaEventElapsedTime(&ms, a, b);
+                    cudaEventDestroy(a);
+                    cudaEventDestroy(b);
+                    return ms;
+                },
+                convert + upload, convert, upload, "rows");
+        vcsrmc_device_free(hd);
+        vcsrmc_format_free(hf);
+        vcsrmc_csr_free(hc);
+        cudaFree(dQ);
+        cudaFree(dS);
+        cudaFree(dW);
     }
     cudaStreamDestroy(st);
     cudaFree(flush_buf);
