@@ -94,6 +94,7 @@ cudaError_t spmm_rows_mx(const RowPlanView& P, const MxView& B, int O, float* C,
     a.vals = P.vals;
     a.hot_cols = P.hot.hot_cols;
     a.B = B;
+    a.N = P.N;
     a.O = O;
     a.C = C;
     a.ldc = ldc;

@@ -3,10 +3,10 @@
 //
 //   C[i, c] (+)= scale * sum_j a_ij * elem[j, c] * 2^(S[j, c / 32] - 127)      sums in fp32
 //
-// A group of 2, 4 or 8 lanes owns one work unit of the row view (plan_rows.hpp) and one slab of 32, 64 or
-// 128 columns of C; a lane holds 16 columns. Entries are staged eight at a time in shared memory as (column,
-// a * 2^e for each of the slab's blocks), so the scale is applied once per entry and block and not in every
-// lane. The groups of a warp take their steps together (the trip count is the warp's largest), which keeps the
+// A group of 4, 8 or 16 lanes owns one work unit of the row view (plan_rows.hpp) and one slab of 32, 64 or
+// 128 columns of C; a lane holds 8 or 16 columns. Entries are staged 8 or 16 at a time in shared memory as
+// (column, a * 2^e for each of the slab's blocks), so the scale is applied once per entry and block and not in
+// every lane. The groups of a warp take their steps together (the trip count is the warp's largest), which keeps the
 // warp converged. A row of C has one owner and is written once at its last entry; a chunk of a split row goes
 // to a row of the workspace, and the chunks are added up in their order afterwards (join_chunks_kernel):
 // the result does not depend on the order in which the groups run.
@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mx.cuh"
 #include "mx.hpp"
@@ -24,7 +25,6 @@ namespace dev {
 namespace rows_mx {
 
 constexpr int kWarps = 4;  // per block
-constexpr int kBatch = 8;  // entries staged at once
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kNever = 0x7fffffff;
 
@@ -36,12 +36,13 @@ struct Lanes {
     static constexpr int kGroups = 32 / kGroup;            // units per warp
     static constexpr int kSlab = kGroup * kCols;           // columns
     static constexpr int kBlocks = kSlab / kMxBlock;       // scale blocks of the slab
+    static constexpr int kBatch = kGroup > 8 ? kGroup : 8;  // entries staged at once
     static constexpr int kPer = kBatch / kGroup;           // entries a lane stages
 };
 
 // A batch of entries as a group stages it: columns, and for each of the slab's blocks the A values times
 // the block's scale, in fp16 (in the first half of the place) or fp32.
-template <int kBlocks>
+template <int kBlocks, int kBatch>
 struct alignas(16) Stage {
     int col[kBatch];
     uint32_t a[kBlocks][kBatch];
@@ -98,17 +99,19 @@ __device__ __forceinline__ uint32_t pair_of(const uint32_t (&r)[kW], int i) {
     return k4 ? decode2<k4>(r[k4 ? i >> 2 : 0], i & 3) : decode2<k4>(r[k4 ? 0 : i >> 1], i & 1);
 }
 
-// How a lane reads its elements. kWhole: 16 consecutive columns in one aligned load. Else word by word, the
-// words of a row dealt out over the group's lanes in turn, so that a load of the group is one stretch of the
-// row: kWords reads aligned words, kBytes two aligned ones that are shifted into place.
-enum class Access { kWhole, kWords, kBytes };
+// How a lane reads its elements. kWhole: its consecutive columns in one aligned load. kPadded: the same for rows
+// that end inside a load but are far enough apart; the operand's last row is then read word by word, as what
+// follows it may not be the operand's. Else word by word, the words of a row dealt out over the group's lanes in
+// turn, so that a load of the group is one stretch of the row: kWords reads aligned words, kBytes two aligned ones
+// that are shifted into place.
+enum class Access { kWhole, kPadded, kWords, kBytes };
 
 // The columns of a lane: kW words of kIn columns each.
 template <bool k4, class L, Access kAccess>
 struct Columns {
     static constexpr int kIn = k4 ? 8 : 4;
     static constexpr int kW = L::kCols / kIn;
-    static constexpr bool kWhole = kAccess == Access::kWhole;
+    static constexpr bool kWhole = kAccess == Access::kWhole || kAccess == Access::kPadded;
     static constexpr int kScales = kWhole ? 1 : kW;  // scale blocks a lane may touch
     static constexpr int kRun = kWhole ? L::kCols : kIn;  // consecutive columns
     // first column of word i, from the slab's first
@@ -118,10 +121,15 @@ struct Columns {
 // The lane's words of the row at `row`, word i from byte at[i], bytes[i] bytes of which are the row's (and
 // may be read: every aligned word that is read holds one of them).
 template <Access kAccess, int kW, int kAt>
-__device__ __forceinline__ void load_raw(const uint8_t* row, const int (&at)[kAt], const int (&bytes)[kAt], uint32_t (&r)[kW]) {
-    if constexpr (kAccess == Access::kWhole) {
+__device__ __forceinline__ void load_raw(const uint8_t* row, const int (&at)[kAt], const int (&bytes)[kAt], bool last, uint32_t (&r)[kW]) {
+    if constexpr (kAccess == Access::kWhole || kAccess == Access::kPadded) {
         const uint8_t* p = row + at[0];
-        if constexpr (kW == 2) {
+        if (kAccess == Access::kPadded && last && bytes[0] < 4 * kW) {
+#pragma unroll
+            for (int i = 0; i < kW; ++i) r[i] = 4 * i < bytes[0] ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+        } else if constexpr (kW == 1) {
+            r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        } else if constexpr (kW == 2) {
             const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
             r[0] = v.x;
             r[1] = v.y;
@@ -183,7 +191,7 @@ struct Args {
     const void* vals;
     const int* hot_cols;
     MxView B;
-    int O;
+    int N, O;
     float* C;
     int64_t ldc;
     float scale;
@@ -223,9 +231,9 @@ template <bool k4, class L, Access kAccess, bool kVec, typename VT>
 __global__ void __launch_bounds__(kWarps * 32) rows_mx_kernel(Args P) {
     constexpr bool kAcc16 = sizeof(VT) == 2;
     using M = Columns<k4, L, kAccess>;
-    constexpr int kPairs = L::kCols / 2, kBlocks = L::kBlocks, kPer = L::kPer, kFlight = L::kFlight;
+    constexpr int kPairs = L::kCols / 2, kBlocks = L::kBlocks, kPer = L::kPer, kFlight = L::kFlight, kBatch = L::kBatch;
     constexpr int kW = M::kW, kScales = M::kScales;
-    __shared__ Stage<kBlocks> stage_all[2][kWarps * L::kGroups];
+    __shared__ Stage<kBlocks, kBatch> stage_all[2][kWarps * L::kGroups];
     __shared__ int ends_all[kWarps * L::kGroups][kUnitRows + 1];
     const VT* vals = static_cast<const VT*>(P.vals);
     const int lane = threadIdx.x & 31, sub = lane / L::kGroup, sl = lane % L::kGroup;
@@ -241,7 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_mx_kernel(Args P) {
     for (int i = 0; i < kScales; ++i) {
         int c = M::of(sl, i);
         if (c >= exist) c = 0;
-        const int n = min(M::kIn, exist - c);
+        const int n = min(M::kWhole ? L::kCols : M::kIn, exist - c);
         at[i] = k4 ? (slab + c) / 2 : slab + c;
         bytes[i] = k4 ? (n + 1) / 2 : n;
         block[i] = c / kMxBlock;
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_mx_kernel(Args P) {
     // where each row ends
     int* ends = ends_all[group];
 #pragma unroll
-    for (int k = 0; k < kUnitRows / L::kGroup; ++k) {
+    for (int k = 0; k < (kUnitRows + L::kGroup - 1) / L::kGroup; ++k) {
         const int r = sl + k * L::kGroup;
         ends[r] = r >= rows ? kNever : rows == 1 ? n : int(P.rp[u.x + r + 1] - pb);
     }
@@ -338,7 +346,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_mx_kernel(Args P) {
     }
     const int longest = __reduce_max_sync(kFull, n);
     for (int q = 0; q < longest; q += kBatch) {
-        Stage<kBlocks>& stage = stage_all[(q / kBatch) & 1][group];
+        Stage<kBlocks, kBatch>& stage = stage_all[(q / kBatch) & 1][group];
         // A values times the scale of each block; 0 past the unit's end, where the A value and code are 0
         float a[kPer][kBlocks];
 #pragma unroll
@@ -429,7 +437,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_mx_kernel(Args P) {
                 const int4 c = *reinterpret_cast<const int4*>(stage.col + j0 + j);
                 const int cj[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) load_raw<kAccess>(P.B.q + uint64_t(uint32_t(cj[k])) * ldq, at, bytes, raw[j + k]);
+                for (int k = 0; k < 4; ++k) load_raw<kAccess>(P.B.q + uint64_t(uint32_t(cj[k])) * ldq, at, bytes, cj[k] == P.N - 1, raw[j + k]);
             }
             // no group has a row's end among these entries: no test for one after each
             const bool straight = !__any_sync(kFull, end <= q + j0 + kFlight);
@@ -501,21 +509,49 @@ cudaError_t launch(Args a, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-template <bool k4, class L, typename VT>
+// Wide: the form for aligned loads of a whole lane, Narrow for word by word, which takes more registers per column.
+template <bool k4, class Wide, class Narrow, typename VT>
 cudaError_t launch_lanes(const Args& a, cudaStream_t st) {
     const uintptr_t q = reinterpret_cast<uintptr_t>(a.B.q);
-    const int64_t full = k4 ? L::kCols / 2 : L::kCols;
-    if (a.O % L::kCols == 0 && q % full == 0 && a.B.ldq % full == 0) return launch<k4, L, Access::kWhole, VT>(a, st);
-    if (q % 4 == 0 && a.B.ldq % 4 == 0) return launch<k4, L, Access::kWords, VT>(a, st);
-    return launch<k4, L, Access::kBytes, VT>(a, st);
+    const int64_t full = k4 ? Wide::kCols / 2 : Wide::kCols, row_bytes = k4 ? (int64_t(a.O) + 1) / 2 : a.O;
+    if (q % full == 0 && a.B.ldq % full == 0) {
+        if (a.O % Wide::kCols == 0) return launch<k4, Wide, Access::kWhole, VT>(a, st);
+        if (a.B.ldq >= (row_bytes + full - 1) / full * full) return launch<k4, Wide, Access::kPadded, VT>(a, st);
+    }
+    if (q % 4 == 0 && a.B.ldq % 4 == 0) return launch<k4, Narrow, Access::kWords, VT>(a, st);
+    return launch<k4, Narrow, Access::kBytes, VT>(a, st);
 }
 
-// One pair of element and A value types; each pair is a translation unit.
+template <bool k4, typename VT>
+cudaError_t product_columns(const Args& a, cudaStream_t st) {
+    // Columns per lane and entries in flight as measured on 262144 rows of 16 entries, O = 32: 4 lanes of 8 columns 60
+    // (E2M1) and 60 us (E4M3, four in flight; eight: 71), 2 lanes of 16: 74 and 75; O = 64: 8 lanes of 8 columns 67,
+    // 4 of 16 85 us; O = 128: 16 lanes of 8 columns 96, as 8 of 16, but 468 against 409 us on the stencil. Word by
+    // word, O = 300 in 4 bits: 381 against 438 us; O = 100, fp32 A: 129 against 149 us; O = 101 in 8 bits, fp16 A:
+    // 195 against 180 us.
+    if (a.O <= 32) return launch_lanes<k4, Lanes<4, 8, k4 ? 8 : 4>, Lanes<4, 8, k4 ? 8 : 4>, VT>(a, st);
+    if (a.O <= 64) return launch_lanes<k4, Lanes<8, 8, 8>, Lanes<8, 8, 8>, VT>(a, st);
+    using Narrow = typename std::conditional<k4 || sizeof(VT) == 4, Lanes<16, 8, 8>, Lanes<8, 16, 8>>::type;
+    return launch_lanes<k4, Lanes<8, 16, 8>, Narrow, VT>(a, st);
+}
+
+// One pair of element and A value types; each pair is a translation unit. Up to 64 columns behind the last whole slab
+// of 128 go to a launch of their own, whose lanes they fill, where that takes less than the launch.
 template <bool k4, typename VT>
 cudaError_t product(const Args& a, cudaStream_t st) {
-    if (a.O <= 32) return launch_lanes<k4, Lanes<2, 16, 4>, VT>(a, st);
-    if (a.O <= 64) return launch_lanes<k4, Lanes<4, 16, 8>, VT>(a, st);
-    return launch_lanes<k4, Lanes<8, 16, 8>, VT>(a, st);
+    const int rest = a.O % 128;
+    if (a.O < 128 || rest == 0 || rest > 64 || a.n_units < 8192) return product_columns<k4, VT>(a, st);
+    Args b = a;
+    const int c = a.O - rest;
+    b.O = rest;
+    b.B.q += k4 ? c / 2 : c;
+    b.B.s += c / kMxBlock;
+    b.C += c;
+    b.partial += c;
+    Args head = a;
+    head.O = c;
+    const cudaError_t e = product_columns<k4, VT>(head, st);
+    return e != cudaSuccess ? e : product_columns<k4, VT>(b, st);
 }
 
 extern template cudaError_t product<true, __half>(const Args&, cudaStream_t);
