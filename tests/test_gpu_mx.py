@@ -583,3 +583,29 @@ def test_driver_microscaled(cuda, O):
     assert all(r["validation"] == "pass" and float(r["gbps_alg"]) > 0 for r in rows.values())
     # fp16 values of A are all that is rounded: half a step of 2^-11 at most, and the check's bound of 3e-3 is far
     assert all(float(rows[k]["rel_l2"]) <= 2.0 ** -11 for k in ("vcsr_mc_mxf8", "vcsr_mc_mxf4"))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("O", [64, 100, 512, 1056])
+def test_norm_scales_at_their_borders(cuda, kind, O):
+    """Blocks whose largest value lies within a few units of fp32's last place of the border between two scales: the scale is the
+    64-bit definition's, for every block (64-bit sums and three 64-bit roundings reach 2^-50, and no value is built nearer than 2^-40)."""
+    rng = np.random.default_rng(O)
+    rows, top = 600, ref.LARGEST[kind]
+    x = rng.standard_normal((rows, O)).astype(np.float32)
+    w = (1 + 0.1 * rng.standard_normal(O)).astype(np.float32)
+    # column 3 holds the first block's largest value, at the border's value T but for a few 2^-24: x with x w / sqrt((S + x^2) / O + eps) = T
+    x[:, :32] *= 0.2
+    border = top * 2.0 ** np.ceil(np.log2(1.4 / top))
+    T = border * (1 + rng.integers(-4, 5, rows) * 2.0 ** -24) / w[3].astype(np.float64)
+    S = (np.delete(x, 3, 1).astype(np.float64) ** 2).sum(1)
+    x[:, 3] = T * np.sqrt((S + O * 1e-6) / (O - T * T))
+    y, _ = ref.norm(x, w, 1e-6)
+    amax = np.abs(y[:, :32]).max(1)
+    off = np.abs(amax / border - 1)
+    keep = off > 2.0 ** -40
+    Q, _, _ = vm.add_rms_norm(torch.from_numpy(x).cuda(), torch.from_numpy(w).cuda(), eps=1e-6, kind=KINDS[kind])
+    codes, scales = codes_of(Q)
+    assert np.array_equal(scales[keep, 0], ref.scale_codes(y, kind)[keep, 0])
+    check_norm(Q, torch.from_numpy(1 / np.sqrt((x.astype(np.float64) ** 2).mean(1) + 1e-6)).cuda().float(), torch.from_numpy(x), torch.from_numpy(w), 1e-6, kind)
+    assert (off < 2.0 ** -21).sum() > 50, "too few rows at the border"

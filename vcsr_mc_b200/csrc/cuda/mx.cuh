@@ -111,6 +111,18 @@ __device__ __forceinline__ void store8(T* p, int nv, bool vec, const float (&v)[
     }
 }
 
+// Two elements, `lo` in the low half of the result (8 bits of it for E2M1, 16 for E4M3).
+__device__ __forceinline__ uint32_t mx_encode2_e2m1(float lo, float hi) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ uint32_t mx_encode2_e4m3(float lo, float hi) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
 // Largest |x| of the two and `m`; a NaN wins.
 __device__ __forceinline__ float max3_abs(float m, float x, float y) {
     asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(x), "f"(y));
@@ -120,12 +132,15 @@ __device__ __forceinline__ float max3_abs(float m, float x, float y) {
 // Quantises and stores eight columns of a block held by four neighbouring lanes (8 columns each; all
 // 32 lanes of the warp take part). `q` is the eight columns' place in the row (byte c for E4M3, c / 2 for
 // E2M1), `s` the block's scale; nv of the eight columns exist (0: nothing is stored), the others are zeros.
-// `vec`: q is aligned to its full store (8 bytes for E4M3, 4 for E2M1).
-__device__ __forceinline__ void mx_store_block(const float (&y)[8], int nv, bool q4, uint8_t* q, uint8_t* s, bool vec) {
+// `vec`: q is aligned to its full store (8 bytes for E4M3, 4 for E2M1). True where the block's largest magnitude
+// is within four units of the last place of a border between two scales: a y that was rounded on its way may then
+// stand on the wrong side of it (one block in a million).
+__device__ __forceinline__ bool mx_store_block(const float (&y)[8], int nv, bool q4, uint8_t* q, uint8_t* s, bool vec) {
     uint32_t amax = __float_as_uint(max3_abs(max3_abs(max3_abs(max3_abs(0.f, y[0], y[1]), y[2], y[3]), y[4], y[5]), y[6], y[7]));
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    if (nv <= 0) return;
+    const bool near = (amax & 0x7fffffu) - ((q4 ? 0x400000u : 0x600000u) - 4u) <= 8u;
+    if (nv <= 0) return false;
     const uint32_t code = mx_scale_code(amax, q4);
     if ((threadIdx.x & 3) == 0) *s = uint8_t(code);
     const float inv = mx_inverse_scale(code);  // of no use in a block with the NaN scale
@@ -164,6 +179,7 @@ __device__ __forceinline__ void mx_store_block(const float (&y)[8], int nv, bool
                 if (i < nv) q[i] = uint8_t(w[i >> 2] >> (8 * (i & 3)));
         }
     }
+    return near;
 }
 
 // From columns dealt out over kL neighbouring lanes (t[j] is column j * kL + lane of a span of 8 * kL, as coalesced

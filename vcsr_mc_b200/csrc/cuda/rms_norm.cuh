@@ -38,6 +38,10 @@ struct Span {
     static constexpr int kThreads = kThreads_;     // per block, at most
     static constexpr int kRows = kL_ ? 256 / (kL_ ? kL_ : 1) : 1;  // rows in a block
     static constexpr int kW = kL_ ? kL_ : 32;      // threads whose groups are neighbours
+    // forward blocks per SM that the registers are held to: with eight columns a thread, all of an SM's threads (2^20
+    // rows of 128: 191 against 202 us); with 16 in blocks of up to 512, three blocks (16384 rows of 4096: 110 against
+    // 115 us with four and 122 with two)
+    static constexpr int kForwardBlocks = !kAny && kN == 8 ? 2048 / kThreads : kThreads == 512 ? 3 : 1;
     static_assert(kN % 8 == 0, "whole groups");
     __device__ static int per_row() { return kL ? kL : int(blockDim.x); }
     __device__ static int slot() { return kL ? int(threadIdx.x) % (kL ? kL : 1) : int(threadIdx.x); }
@@ -163,19 +167,65 @@ __device__ __forceinline__ T row_sum(T v, T* smem) {
     return v;
 }
 
-// 1 / sqrt(v), rounded once to fp32: the hardware's estimate and a Newton step in 64 bits (its error squared,
+// 1 / sqrt(v): the hardware's estimate and a Newton step in 64 bits (its error squared,
 // below 2^-40), or 64-bit operations where v leaves the estimate's range.
-__device__ __forceinline__ float inverse_root(double v) {
+__device__ __forceinline__ double inverse_root(double v) {
     if (v > 1e-30 && v < 1e30) {
         const double r = double(rsqrtf(float(v)));
-        return float(r * (1.5 - 0.5 * v * r * r));
+        return r * (1.5 - 0.5 * v * r * r);
     }
-    return float(1.0 / sqrt(v));
+    return 1.0 / sqrt(v);
+}
+
+__device__ __forceinline__ float read_as(const DenseView& d, int64_t row, int c) {
+    const int64_t i = row * d.ld + c;
+    if (d.dtype == VCSRMC_F32) return static_cast<const volatile float*>(d.p)[i];
+    const unsigned short h = static_cast<const volatile unsigned short*>(d.p)[i];
+    return d.dtype == VCSRMC_F16 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
+}
+
+// Writes the block from column c on again, its scale from the largest |s * root * w| in 64 bits: for a block whose
+// largest value in fp32 is next to a border between scales. One thread, from memory, and a call of its own: a block
+// in a million needs it, and in the kernel's registers it would cost all of them (218 against 191 us for 2^20 rows
+// of 128).
+static __device__ __noinline__ void rewrite_block(const RmsNormArgs& a, int64_t row, int c, double root) {
+    const float inv = float(root);
+    const DenseView weight{const_cast<void*>(a.weight), a.w_dtype, 0};
+    const int n = min(kMxBlock, a.O - c);
+    auto sum = [&](int i) {
+        if (a.residual_out.p) return read_as(a.residual_out, row, c + i);
+        const float v = read_as(a.x, row, c + i) + (a.residual.p ? read_as(a.residual, row, c + i) : 0.f);
+        if (a.residual_out.dtype == VCSRMC_F32) return v;
+        return a.residual_out.dtype == VCSRMC_F16 ? __half2float(__float2half_rn(v)) : __bfloat162float(__float2bfloat16_rn(v));
+    };
+    double exact = 0.0;
+    float amax = 0.f;
+    for (int i = 0; i < n; ++i) {
+        const float v = sum(i), w = read_as(weight, 0, c + i);
+        exact = fmax(exact, fabs(double(v) * root * double(w)));
+        amax = fmaxf(amax, fabsf(v * inv * w));
+    }
+    const uint32_t border = (__float_as_uint(amax) & 0x7f800000u) | (a.out.q4 ? 0x400000u : 0x600000u);
+    const uint32_t code = mx_scale_code(exact > double(__uint_as_float(border)) ? border + 1u : border, a.out.q4);
+    const float scale = mx_inverse_scale(code);
+    uint8_t* q = a.out.q + row * a.out.ldq;
+    a.out.s[row * a.out.lds + c / kMxBlock] = uint8_t(code);
+    for (int i = 0; i < n; i += 2) {
+        float y[2] = {0.f, 0.f};
+        for (int k = 0; k < 2 && i + k < n; ++k) y[k] = sum(i + k) * inv * read_as(weight, 0, c + i + k) * scale;
+        if (a.out.q4) {
+            q[(c + i) / 2] = uint8_t(mx_encode2_e2m1(y[0], y[1]));
+        } else {
+            const uint32_t two = mx_encode2_e4m3(y[0], y[1]);
+            q[c + i] = uint8_t(two);
+            if (i + 1 < n) q[c + i + 1] = uint8_t(two >> 8);
+        }
+    }
 }
 
 template <class S, bool kXWide, bool kRWide>
-__global__ void __launch_bounds__(S::kThreads) rms_norm_kernel(RmsNormArgs a) {
-    __shared__ double smem[32];
+__global__ void __launch_bounds__(S::kThreads, S::kForwardBlocks) rms_norm_kernel(const __grid_constant__ RmsNormArgs a) {
+    __shared__ double smem[32], roots[S::kL ? S::kRows : 32];
     extern __shared__ __align__(16) float turn[];  // kV = 1: eight floats a thread
     const int64_t row = int64_t(blockIdx.x) * S::kRows + S::row_in_block();
     const bool live = row < a.rows;  // every thread takes part in the reductions of a row past the end
@@ -209,7 +259,11 @@ __global__ void __launch_bounds__(S::kThreads) rms_norm_kernel(RmsNormArgs a) {
         for (int i = 0; i < S::kN; ++i) sum = fma(double(s[i]), double(s[i]), sum);
     }
     sum = row_sum<S>(sum, smem);
-    const float inv = inverse_root(sum / double(a.O) + double(a.eps));
+    const double root = inverse_root(sum / double(a.O) + double(a.eps));
+    const float inv = float(root);
+    // for rewrite_block, kept out of the registers; one for a warp's own use where it shares a row
+    const int root_at = S::kL ? S::row_in_block() : int(threadIdx.x >> 5);
+    if (S::slot() % 32 == 0) roots[root_at] = root;
     if (live && S::slot() == 0 && a.inv_rms) a.inv_rms[row] = inv;
     uint8_t* q = a.out.q + row * a.out.ldq;
     uint8_t* scales = a.out.s + row * a.out.lds;
@@ -218,18 +272,27 @@ __global__ void __launch_bounds__(S::kThreads) rms_norm_kernel(RmsNormArgs a) {
         if (a.residual_out.p) store<S, kRWide>(s, a.residual_out, row, O, k);
         float w[S::kN];
         load_weights<S>(w, a.weight, a.w_dtype, a.vec_w, O, k);
+        uint32_t again = 0;  // groups whose block is next to a border between scales
 #pragma unroll
         for (int i = 0; i < S::kN; i += 8) {
             float y[8], t[8];
+            bool near;
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[j] = s[i + j] * inv * w[i + j];
             const int c = S::group(i / 8, k);
             if constexpr (S::kV == 1) {
                 turn_to_groups<S::kW>(t, y, turn + 8 * (threadIdx.x - S::slot() % S::kW), S::slot() % S::kW);
-                mx_store_block(y, max(0, min(8, O - c)), a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock, a.vec_q);
+                near = mx_store_block(y, max(0, min(8, O - c)), a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock, a.vec_q);
             } else {
-                mx_store_block(t, c < O ? 8 : 0, a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock, true);
+                near = mx_store_block(t, c < O ? 8 : 0, a.out.q4, q + (a.out.q4 ? c / 2 : c), scales + c / kMxBlock, true);
             }
+            if (near) again |= 1u << (i / 8);
+        }
+        if (__any_sync(0xffffffffu, again != 0)) {
+            __syncwarp();  // the block's values and first bytes are written
+            if (S::slot() % 4 == 0)
+                for (int g = 0; g < S::kN / 8; ++g)
+                    if ((again >> g) & 1u) rewrite_block(a, row, S::group(g, k), roots[root_at]);
         }
     }
 }
