@@ -338,7 +338,7 @@ def test_product_refusals(cuda):
             call()
     from vcsr_mc_b200 import _lib
     with pytest.raises(vm.VcsrmcError):  # no workspace for the split row
-        _lib.call("vcsrmc_spmm_mx", dV.handle, *Q._args(), 64, C.data_ptr(), 64, 0, None, 0, None)
+        _lib.call("vcsrmc_spmm_mx", dV.handle, Q.data.data_ptr(), Q.kind, 64, Q.scale.data_ptr(), 2, 64, C.data_ptr(), 64, 0, None, 0, None)
     only_segment = vm.upload_vcsr_mc_device(vm.csr_to_vcsr_mc(vm.CSR.from_arrays(M, N, *csr), segw=32), plans=[vm.PLAN_SEGMENT])
     with pytest.raises(vm.VcsrmcError):
         vm.spmm(only_segment, Q, C)

@@ -14,9 +14,7 @@ every computation runs in libvcsrmc.so.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-import functools
 from typing import Optional
 
 import numpy as np
@@ -203,7 +201,6 @@ class DeviceVCSRMC:
     def __init__(self, handle: ctypes.c_void_p, host: Optional[VCSRMC], device: int, **shape):
         self._h = handle
         self.device = device
-        self._mx_workspace = {}
         if host is not None:
             shape = dict(M=host.M, N=host.N, fp32=host.fp32, scale=host.scale, segw=host.segw)
         self.M, self.N, self.fp32, self.scale, self.segw = (shape[k] for k in ("M", "N", "fp32", "scale", "segw"))
@@ -225,15 +222,6 @@ class DeviceVCSRMC:
     @property
     def handle(self) -> ctypes.c_void_p:
         return self._h
-
-    def mx_workspace(self, O: int) -> int:
-        """Bytes of workspace of a product with O columns of a microscaled B (vcsrmc_spmm_mx_workspace)."""
-        n = self._mx_workspace.get(O)
-        if n is None:
-            size = ctypes.c_int64()
-            call("vcsrmc_spmm_mx_workspace", self._h, O, ctypes.byref(size))
-            n = self._mx_workspace[O] = size.value
-        return n
 
     def free(self) -> None:
         h, self._h = self._h, None
@@ -336,7 +324,6 @@ def spmm(dV: DeviceVCSRMC, B, C, tileK: int = 128, accumulate: bool = False, str
 
 
 MX_BLOCK = 32  # columns of an MX matrix that share a scale
-_NO_GUARD = contextlib.nullcontext()
 
 
 def _invalid(message: str) -> VcsrmcError:
@@ -351,7 +338,7 @@ class MXDense:
     scale: float8_e8m0fnu (or uint8) [rows, ceil(cols / 32)]
     Rows may be strided; columns may not. `cols` is needed for an odd number of MXF4 columns."""
 
-    __slots__ = ("data", "scale", "kind", "rows", "cols", "device", "_ldq", "_lds")
+    __slots__ = ("data", "scale", "kind", "rows", "cols", "_ldq", "_lds")
 
     def __init__(self, data, scale, cols: Optional[int] = None):
         import torch
@@ -372,15 +359,12 @@ class MXDense:
             raise _invalid("the columns of MX elements and scales must be contiguous")
         if data.device != scale.device:
             raise _invalid("MX elements and scales must be on the same device")
-        self._set(data, scale, kind, rows, cols, data.device, _row_stride(data), _row_stride(scale))
+        self.data, self.scale, self.kind, self.rows, self.cols = data, scale, kind, rows, cols
+        self._ldq, self._lds = _row_stride(data), _row_stride(scale)
 
-    def _set(self, data, scale, kind, rows, cols, device, ldq, lds):
-        self.data, self.scale, self.kind, self.rows, self.cols, self.device = data, scale, kind, rows, cols, device
-        self._ldq, self._lds = ldq, lds
-
-    def _args(self):
-        """Pointer, type, row stride, scale pointer and scale row stride, as the C ABI takes them."""
-        return self.data.data_ptr(), self.kind, self._ldq, self.scale.data_ptr(), self._lds
+    @property
+    def device(self):
+        return self.data.device
 
     @property
     def shape(self):
@@ -390,20 +374,28 @@ class MXDense:
     def empty(rows: int, cols: int, kind: int = MXF8, device=None) -> "MXDense":
         """An MXDense to write to. Its rows start at multiples of 16 bytes (those of its scales: 4), whatever `cols` is, so that
         every operator can use its widest loads and stores."""
-        torch = _torch or _load_torch()
-        if kind != MXF8 and kind != MXF4:
+        import torch
+        if kind not in (MXF8, MXF4):
             raise _invalid("the microscaled kind must be MXF8 or MXF4")
-        width, blocks = (cols if kind == MXF8 else (cols + 1) // 2), (cols + MX_BLOCK - 1) // MX_BLOCK
-        ldq, lds = (width + 15) & -16, (blocks + 3) & -4
-        data = torch.empty(rows, ldq, dtype=torch.float8_e4m3fn if kind == MXF8 else torch.uint8, device=device)
-        scale = torch.empty(rows, lds, dtype=torch.float8_e8m0fnu, device=device)
-        if ldq != width:
-            data = data[:, :width]
-        if lds != blocks:
-            scale = scale[:, :blocks]
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise _invalid("microscaled operators run on CUDA tensors")
+        index = torch.cuda.current_device() if device.index is None else device.index
+        data, scale, ldq, lds = (_ops or _load_ops()).mx_empty(rows, cols, kind, index)
+        return MXDense._of(data, scale, kind, rows, cols, ldq, lds)
+
+    @staticmethod
+    def _of(data, scale, kind: int, rows: int, cols: int, ldq: int, lds: int) -> "MXDense":
         out = MXDense.__new__(MXDense)
-        out._set(data, scale, kind, rows, cols, data.device, ldq, lds)
+        out.data, out.scale, out.kind, out.rows, out.cols, out._ldq, out._lds = data, scale, kind, rows, cols, ldq, lds
         return out
+
+    def _args(self):
+        """Elements, scales, kind and the row strides of both, as _torch_ops takes them."""
+        return self.data, self.scale, self.kind, self._ldq, self._lds
+
+
+_NO_MX = (None,) * 5
 
 
 def _row_stride(t) -> int:
@@ -411,131 +403,82 @@ def _row_stride(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
-_torch = None
-_DENSE = {}  # torch dtype -> VCSRMC code
+_ops = None
 
 
-def _load_torch():
-    """torch, imported at the first microscaled call."""
-    global _torch
+def _load_ops():
+    """vcsr_mc_b200._torch_ops (csrc/torch_ops.cpp): checks, allocation and the C ABI call of the microscaled operators. Built in-tree
+    with the library; there is no other path."""
+    global _ops
+    import torch  # noqa: F401  (the module links against it)
+    _lib.lib()
+    try:
+        from . import _torch_ops
+    except ImportError as e:
+        raise ImportError(f"vcsr_mc_b200/_torch_ops.so is not built or does not load ({e}); run `make -C vcsr_mc_b200/csrc`") from e
+    _torch_ops.set_error(VcsrmcError)
+    _ops = _torch_ops
+    return _ops
+
+
+def _stream_guard(stream, device):
+    """torch's guard that makes `stream` (a torch stream, or a raw handle) current on `device`, so that a call's launches and what it
+    allocates belong to it."""
     import torch
-    _DENSE.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-    torch.cuda.is_available() and torch.cuda.init()
-    _torch = torch
-    return torch
-
-
-def _dense(t, what: str):
-    """(pointer, row stride, dtype code, rows, columns, device index) of a dense matrix that an operator takes."""
-    try:
-        rows, cols = t.shape
-        ld, step = t.stride()
-        device = t.get_device()
-        code = _DENSE[t.dtype]
-    except (AttributeError, ValueError, KeyError, TypeError):
-        raise _invalid(f"{what} must be a 2-D float32, float16 or bfloat16 tensor") from None
-    if device < 0:
-        raise _invalid(f"{what} must be a CUDA tensor")
-    if step != 1 and cols > 1:
-        raise _invalid(f"the columns of {what} must be contiguous")
-    if rows <= 1:
-        ld = cols or 1  # torch leaves the stride of a single row open
-    elif ld < cols:
-        raise _invalid(f"the rows of {what} must not overlap")
-    return t.data_ptr(), ld, code, rows, cols, device
-
-
-def _like(t, what: str, rows: int, cols: int, device: int, code: Optional[int] = None):
-    """(pointer, row stride, dtype code) of a matrix that goes with another one: its shape and device, and a type if one is given."""
-    p, ld, c, r, n, d = _dense(t, what)
-    if r != rows or n != cols or d != device:
-        raise _invalid(f"{what} must be {rows} x {cols} on cuda:{device}, with the other tensors")
-    if code is not None and c != code:
-        raise _invalid(f"{what} has another type than the tensors it goes with")
-    return p, ld, c
-
-
-def _vector(t, what: str, device: int, n: int):
-    """(pointer, dtype code) of a contiguous vector of n values."""
-    try:
-        (m,), (step,) = t.shape, t.stride()
-        if m == n and t.get_device() == device and (step == 1 or n <= 1):
-            return t.data_ptr(), _DENSE[t.dtype]
-    except (AttributeError, ValueError, KeyError, TypeError):
-        pass
-    raise _invalid(f"{what} must be a contiguous float32, float16 or bfloat16 tensor of {n} values on cuda:{device}")
-
-
-def _on(torch, device: int, stream):
-    """(guard, stream handle): the guard makes `device` and `stream` (None: torch's current one there) current, so that what is
-    allocated under it belongs to the stream that uses it; it is None where they are current already."""
-    if stream is None:
-        guard = torch.cuda.device(device) if torch._C._cuda_getDevice() != device else None
-        return guard, torch._C._cuda_getCurrentRawStream(device)
+    if device.type != "cuda":
+        raise _invalid("microscaled operators run on CUDA tensors")
     if not isinstance(stream, torch.cuda.Stream):
         raw = int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
         stream = torch.cuda.ExternalStream(raw, device=device)
-    if stream.device.index != device:
-        raise _invalid(f"the stream must be on cuda:{device}, with the tensors")
-    return torch.cuda.stream(stream), stream.cuda_stream
+    if stream.device != device:
+        raise _invalid(f"the stream must be on {device}, with the tensors")
+    return torch.cuda.stream(stream)
 
 
-def _out_mx(out: Optional[MXDense], rows: int, cols: int, kind: int, device) -> MXDense:
+def _mx_out(out: Optional[MXDense], X, kind: int):
     if out is None:
-        return MXDense.empty(rows, cols, kind, device)
-    if out.kind != kind or out.rows != rows or out.cols != cols or out.device != device:
+        return _NO_MX
+    if out.kind != kind or out.shape != tuple(X.shape) or out.device != X.device:
         raise _invalid("out must have X's shape and device, and the kind that is asked for")
-    return out
+    return out._args()
 
 
 def _spmm_mx(dV: DeviceVCSRMC, B: MXDense, C, tileK: int, accumulate: bool, stream, O: Optional[int], plan: int):
-    torch = _torch or _load_torch()
-    c, ldc, c_dtype, rows, cols, device = _dense(C, "C")
-    O = B.cols if O is None else O
-    if c_dtype != F32:
-        raise _invalid("C must be float32")
-    if device != dV.device or B.device.type != "cuda" or B.device.index != device:
-        raise _invalid("A, B and C must be on the same device")
+    if stream is not None:
+        with _stream_guard(stream, C.device):
+            return _spmm_mx(dV, B, C, tileK, accumulate, None, O, plan)
     if plan != PLAN_AUTO and plan != PLAN_ROWS:
         raise _invalid("a microscaled B runs on the ROWS plan")
     if tileK not in (16, 32, 64, 128, 256):
         raise _invalid("tileK must be one of 16, 32, 64, 128, 256")
-    if B.cols < O or cols < O or B.rows < dV.N or rows < dV.M:
-        raise _invalid("B and C must hold A's columns and rows, with >= O columns")
-    guard, st = _on(torch, device, stream)
-    n = dV.mx_workspace(O)
-    with guard or _NO_GUARD:
-        ws = torch.empty(n, dtype=torch.uint8, device=C.device) if n else None
-        call("vcsrmc_spmm_mx", dV.handle, *B._args(), O, c, ldc, 1 if accumulate else 0, ws.data_ptr() if n else None, n, st)
+    h = dV._h
+    (_ops or _load_ops()).spmm_mx(h.value if h else 0, dV.device, dV.M, dV.N, *B._args(), B.rows, B.cols, B.cols if O is None else O, C,
+                                  1 if accumulate else 0)
     return C
 
 
 def mx_quantize(X, kind: int = MXF8, out: Optional[MXDense] = None, stream=None) -> MXDense:
     """X (float32, float16 or bfloat16) in 8 (MXF8) or 4 bits (MXF4): the scale of 32 columns is the smallest power of two
     under which their largest magnitude fits the element type; elements are rounded to nearest, ties to even."""
-    torch = _torch or _load_torch()
-    x, ldx, x_dtype, rows, cols, device = _dense(X, "X")
-    guard, st = _on(torch, device, stream)
-    with guard or _NO_GUARD:
-        Q = _out_mx(out, rows, cols, kind, X.device)
-        q, q_dtype, ldq, s, lds = Q._args()
-        call("vcsrmc_mx_quantize", x, x_dtype, ldx, rows, cols, q_dtype, q, ldq, s, lds, st)
-    return Q
+    if stream is not None:
+        with _stream_guard(stream, X.device):
+            return mx_quantize(X, kind, out)
+    data, scale, ldq, lds = (_ops or _load_ops()).mx_quantize(X, kind, *_mx_out(out, X, kind))
+    return MXDense._of(data, scale, kind, *X.shape, ldq, lds) if out is None else out
 
 
 def mx_dequantize(Q: MXDense, dtype=None, out=None, stream=None):
     """The values an MXDense stands for, rounded to `dtype` (default float32)."""
-    torch = _torch or _load_torch()
-    if Q.device.type != "cuda":
-        raise _invalid("Q must be on a CUDA device")
-    guard, st = _on(torch, Q.device.index, stream)
-    with guard or _NO_GUARD:
-        Y = torch.empty(Q.rows, Q.cols, dtype=dtype or torch.float32, device=Q.device) if out is None else out
-        if dtype is not None and Y.dtype != dtype:
-            raise _invalid(f"out must be {dtype}, got {Y.dtype}")
-        y, ldy, y_dtype = _like(Y, "out", Q.rows, Q.cols, Q.device.index)
-        call("vcsrmc_mx_dequantize", *Q._args(), Q.rows, Q.cols, y, y_dtype, ldy, st)
-    return Y
+    if stream is not None:
+        with _stream_guard(stream, Q.device):
+            return mx_dequantize(Q, dtype, out)
+    import torch
+    if out is None:
+        out = torch.empty(Q.rows, Q.cols, dtype=dtype or torch.float32, device=Q.data.device)
+    elif dtype is not None and out.dtype != dtype:
+        raise _invalid(f"out must be {dtype}, got {out.dtype}")
+    (_ops or _load_ops()).mx_dequantize(*Q._args(), Q.rows, Q.cols, out)
+    return out
 
 
 def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, out: Optional[MXDense] = None, residual_out=None,
@@ -543,61 +486,21 @@ def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, 
     """(Q, residual_out, inv_rms): s = X + residual, rounded to the residual's type (residual_out); inv_rms = 1 / sqrt(mean(s^2) +
     eps) of every row (float32); Q = MX(s * inv_rms * weight). The residual has X's type, or X is float32 (a product's C). Without a
     residual s is X, which is then returned in residual_out's place. residual_out may be the residual, or X of the same type (in place)."""
-    torch = _torch or _load_torch()
-    x, ldx, x_dtype, rows, cols, device = _dense(X, "X")
-    w, w_dtype = _vector(weight, "weight", device, cols)
-    r, ldr, r_dtype = (None, 0, x_dtype) if residual is None else _like(residual, "residual", rows, cols, device)
-    at = X.device
-    guard, st = _on(torch, device, stream)
-    with guard or _NO_GUARD:
-        o, ldo = None, 0
-        if residual_out is not None:
-            o, ldo, _ = _like(residual_out, "residual_out", rows, cols, device, r_dtype)
-        elif residual is not None:
-            residual_out = torch.empty(rows, cols, dtype=residual.dtype, device=at)
-            o, ldo = residual_out.data_ptr(), cols
-        Q = _out_mx(out, rows, cols, kind, at)
-        inv_rms = torch.empty(rows, dtype=torch.float32, device=at)
-        q, q_dtype, ldq, s, lds = Q._args()
-        call("vcsrmc_add_rms_norm", x, x_dtype, ldx, r, ldr, o, ldo, r_dtype, w, w_dtype, eps, rows, cols, q_dtype, q, ldq, s, lds,
-             inv_rms.data_ptr(), st)
-    return Q, X if residual_out is None else residual_out, inv_rms
+    if stream is not None:
+        with _stream_guard(stream, X.device):
+            return add_rms_norm(X, weight, residual, eps, kind, out, residual_out)
+    data, scale, ldq, lds, hidden, inv_rms = (_ops or _load_ops()).add_rms_norm(X, weight, residual, eps, kind, *_mx_out(out, X, kind), residual_out)
+    return MXDense._of(data, scale, kind, *X.shape, ldq, lds) if out is None else out, hidden if residual_out is None else residual_out, inv_rms
 
 
 def add_rms_norm_backward(dY, weight, hidden, inv_rms, d_residual=None, out=None, stream=None):
     """(dX, dweight) of add_rms_norm: dY is the gradient of the values Q stands for (float32 or hidden's type; the elements' rounding
     counts as the identity), hidden and inv_rms are what the forward call returned, d_residual the gradient of its residual_out. dX, in
     hidden's type, is the gradient of X and of the residual; dweight is float32. out (dX) may be d_residual, or dY of the same type."""
-    torch = _torch or _load_torch()
-    dy, lddy, dy_dtype, rows, cols, device = _dense(dY, "dY")
-    w, w_dtype = _vector(weight, "weight", device, cols)
-    h, ldh, r_dtype = _like(hidden, "hidden", rows, cols, device)
-    inv, inv_dtype = _vector(inv_rms, "inv_rms", device, rows)
-    if inv_dtype != F32:
-        raise _invalid("inv_rms must be float32")
-    dr, lddr, _ = (None, 0, 0) if d_residual is None else _like(d_residual, "d_residual", rows, cols, device, r_dtype)
-    at = dY.device
-    guard, st = _on(torch, device, stream)
-    with guard or _NO_GUARD:
-        if out is None:
-            out = torch.empty(rows, cols, dtype=hidden.dtype, device=at)
-            dx, lddx = out.data_ptr(), cols
-        else:
-            dx, lddx, _ = _like(out, "out", rows, cols, device, r_dtype)
-        dweight = torch.empty(cols, dtype=torch.float32, device=at)
-        n = _grad_workspace(rows, cols, device)
-        ws = torch.empty(n, dtype=torch.uint8, device=at)
-        call("vcsrmc_add_rms_norm_backward", dy, dy_dtype, lddy, dr, lddr, h, ldh, r_dtype, w, w_dtype, inv, rows, cols, dx, lddx,
-             dweight.data_ptr(), ws.data_ptr(), n, st)
-    return out, dweight
-
-
-@functools.lru_cache(maxsize=256)
-def _grad_workspace(rows: int, cols: int, device: int) -> int:
-    """Bytes of add_rms_norm_backward's workspace; they depend on the shape and the device's SM count."""
-    n = ctypes.c_int64()
-    call("vcsrmc_add_rms_norm_backward_workspace", rows, cols, ctypes.byref(n))
-    return n.value
+    if stream is not None:
+        with _stream_guard(stream, dY.device):
+            return add_rms_norm_backward(dY, weight, hidden, inv_rms, d_residual, out)
+    return (_ops or _load_ops()).add_rms_norm_backward(dY, weight, hidden, inv_rms, d_residual, out)
 
 
 def run_vcsr_mc_spmm_gpu(dV: DeviceVCSRMC, B, O: int, tileK: int, C, stream=None, accumulate: bool = True) -> float:
