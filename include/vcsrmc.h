@@ -288,7 +288,8 @@ int vcsrmc_spmm_mx(const vcsrmc_device_format* d, const void* Q, int q_dtype, in
 /* Between two products: s = X + residual, rounded to the residual's type and stored in residual_out;
  * inv_rms = 1 / sqrt(mean(s^2) + eps) of every row; Q = MX(s * inv_rms * weight). The residual (r_dtype)
  * has X's type, or X is fp32, as a product's C. residual NULL: s = X; residual_out or inv_rms NULL: not
- * stored. residual_out may be residual, or X where the types are the same, with the same stride. */
+ * stored. residual_out may be residual, or X where the types are the same, with the same stride. Values
+ * are computed in fp32 from 64-bit square sums; the scale of a block is that of the 64-bit values. */
 int vcsrmc_add_rms_norm(const void* X, int x_dtype, int64_t ldx, const void* residual, int64_t ldr,
                         void* residual_out, int64_t ldo, int r_dtype, const void* weight, int w_dtype,
                         float eps, int64_t rows, int32_t O, int q_dtype, void* Q, int64_t ldq,

@@ -88,26 +88,21 @@ __device__ __forceinline__ void load8(const T* p, int nv, bool vec, float (&v)[8
         for (int i = 0; i < 8; ++i) v[i] = i < nv ? to_f32(p[i]) : 0.f;
     }
 }
+// Stores eight consecutive elements; p is 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int nv, bool vec, const float (&v)[8]) {
-    if (vec && nv == 8) {
-        if constexpr (sizeof(T) == 4) {
-            __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
-            __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
-        } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                T* h = reinterpret_cast<T*>(&w[i]);
-                h[0] = from_f32<T>(v[2 * i]);
-                h[1] = from_f32<T>(v[2 * i + 1]);
-            }
-            __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
-        }
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+        __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
     } else {
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < nv) p[i] = from_f32<T>(v[i]);
+        for (int i = 0; i < 4; ++i) {
+            T* h = reinterpret_cast<T*>(&w[i]);
+            h[0] = from_f32<T>(v[2 * i]);
+            h[1] = from_f32<T>(v[2 * i + 1]);
+        }
+        __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
     }
 }
 

@@ -1,7 +1,9 @@
 // Quantisation of a dense matrix to the microscaled format, and back (mx.cuh has the format).
 //
 // Both are one pass over memory: per element they move the dense value (2 or 4 bytes) and 1 or 1/2
-// byte of element plus 1/32 byte of scale, so HBM bounds them. A thread owns eight consecutive columns
+// byte of element plus 1/32 byte of scale, so HBM bounds them: 2^20 x 128 fp16 to E2M1 and back to bf16 take 129 us in
+// all on a B200 (675 MB with the 4-bit matrix in between, 5.2 TB/s; copies run at 6.5), 131072 x 512 fp32 to E4M3
+// 52 us (6.6 TB/s, part of it from L2), x 501 bf16, whose rows are not aligned, 64 us. A thread owns eight consecutive columns
 // (16 or 32 bytes of the dense side in flight), four neighbouring threads a block of 32.
 #include <cuda_runtime.h>
 
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(MxView Q, Shape
     }
 #pragma unroll
     for (int k = 0; k < kDequantizeParts; ++k)
-        if (live[k]) store8(Y + int64_t(row[k]) * ldy + c[k], 8, true, v[k]);
+        if (live[k]) store8(Y + int64_t(row[k]) * ldy + c[k], v[k]);
 }
 
 template <typename T, int kL>
