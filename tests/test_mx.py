@@ -114,3 +114,13 @@ def test_python_refusals():
                  lambda: vm.add_rms_norm_backward(torch.zeros(4, 4), torch.zeros(4), torch.zeros(4, 4), torch.zeros(4))):
         with pytest.raises(vm.VcsrmcError):
             make()
+
+
+def test_mx_matrix_is_what_was_checked():
+    """The tensors and the shape of an MXDense stay those that its constructor checked."""
+    Q = vm.MXDense(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8), cols=63)
+    assert (Q.rows, Q.cols, Q.shape, Q.kind, Q.device) == (4, 63, (4, 63), vm.MXF4, torch.device("cpu"))
+    for name, value in (("data", torch.zeros(1, 1, dtype=torch.uint8)), ("scale", torch.zeros(1, 1, dtype=torch.uint8)), ("rows", 9), ("cols", 999),
+                        ("kind", vm.MXF8), ("shape", (9, 9)), ("anything", 1)):
+        with pytest.raises(AttributeError):
+            setattr(Q, name, value)

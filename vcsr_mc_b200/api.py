@@ -336,9 +336,10 @@ class MXDense:
     data:  float8_e4m3fn [rows, cols] (MXF8), or uint8 [rows, ceil(cols / 2)] with two E2M1 elements per
            byte, the even column in the low half (MXF4)
     scale: float8_e8m0fnu (or uint8) [rows, ceil(cols / 32)]
-    Rows may be strided; columns may not. `cols` is needed for an odd number of MXF4 columns."""
+    Rows may be strided; columns may not. `cols` is needed for an odd number of MXF4 columns. The tensors and the shape are set
+    once, so that what was checked here is what the kernels get; the tensors' values may change."""
 
-    __slots__ = ("data", "scale", "kind", "rows", "cols", "_ldq", "_lds")
+    __slots__ = ("_data", "_scale", "_kind", "_rows", "_cols", "_ldq", "_lds")
 
     def __init__(self, data, scale, cols: Optional[int] = None):
         import torch
@@ -359,16 +360,16 @@ class MXDense:
             raise _invalid("the columns of MX elements and scales must be contiguous")
         if data.device != scale.device:
             raise _invalid("MX elements and scales must be on the same device")
-        self.data, self.scale, self.kind, self.rows, self.cols = data, scale, kind, rows, cols
+        self._data, self._scale, self._kind, self._rows, self._cols = data, scale, kind, rows, cols
         self._ldq, self._lds = _row_stride(data), _row_stride(scale)
 
-    @property
-    def device(self):
-        return self.data.device
-
-    @property
-    def shape(self):
-        return (self.rows, self.cols)
+    data = property(lambda self: self._data)
+    scale = property(lambda self: self._scale)
+    kind = property(lambda self: self._kind)
+    rows = property(lambda self: self._rows)
+    cols = property(lambda self: self._cols)
+    shape = property(lambda self: (self._rows, self._cols))
+    device = property(lambda self: self._data.device)
 
     @staticmethod
     def empty(rows: int, cols: int, kind: int = MXF8, device=None) -> "MXDense":
@@ -387,12 +388,12 @@ class MXDense:
     @staticmethod
     def _of(data, scale, kind: int, rows: int, cols: int, ldq: int, lds: int) -> "MXDense":
         out = MXDense.__new__(MXDense)
-        out.data, out.scale, out.kind, out.rows, out.cols, out._ldq, out._lds = data, scale, kind, rows, cols, ldq, lds
+        out._data, out._scale, out._kind, out._rows, out._cols, out._ldq, out._lds = data, scale, kind, rows, cols, ldq, lds
         return out
 
     def _args(self):
         """Elements, scales, kind and the row strides of both, as _torch_ops takes them."""
-        return self.data, self.scale, self.kind, self._ldq, self._lds
+        return self._data, self._scale, self._kind, self._ldq, self._lds
 
 
 _NO_MX = (None,) * 5
@@ -452,7 +453,7 @@ def _spmm_mx(dV: DeviceVCSRMC, B: MXDense, C, tileK: int, accumulate: bool, stre
     if tileK not in (16, 32, 64, 128, 256):
         raise _invalid("tileK must be one of 16, 32, 64, 128, 256")
     h = dV._h
-    (_ops or _load_ops()).spmm_mx(h.value if h else 0, dV.device, dV.M, dV.N, *B._args(), B.rows, B.cols, B.cols if O is None else O, C,
+    (_ops or _load_ops()).spmm_mx(h.value if h else 0, dV.device, dV.M, dV.N, *B._args(), B._rows, B._cols, B._cols if O is None else O, C,
                                   1 if accumulate else 0)
     return C
 
