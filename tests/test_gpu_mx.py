@@ -609,3 +609,119 @@ def test_norm_scales_at_their_borders(cuda, kind, O):
     assert np.array_equal(scales[keep, 0], ref.scale_codes(y, kind)[keep, 0])
     check_norm(Q, torch.from_numpy(1 / np.sqrt((x.astype(np.float64) ** 2).mean(1) + 1e-6)).cuda().float(), torch.from_numpy(x), torch.from_numpy(w), 1e-6, kind)
     assert (off < 2.0 ** -21).sum() > 50, "too few rows at the border"
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("x,r", [("f32", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("O", [8, 40, 96, 264, 1032, 4104])
+def test_norm_in_odd_places(cuda, kind, x, r, O):
+    """Every operand at an odd offset of a larger buffer (the weight and the MX matrix too), forward and backward; what lies around them stays."""
+    rows, g = 37, torch.Generator("cuda").manual_seed(O)
+
+    def place(t, fill):
+        big = torch.full((t.shape[0] + 2, t.shape[1] + 5), fill, dtype=t.dtype, device="cuda")
+        view = big[1:-1, 3:3 + t.shape[1]]
+        view.copy_(t)
+        return big, view
+
+    X = place(torch.randn(rows, O, device="cuda", generator=g).to(TYPES[x]), 7)[1]
+    R = place(torch.randn(rows, O, device="cuda", generator=g).to(TYPES[r]), 7)[1]
+    w = (1 + 0.2 * torch.randn(O + 1, device="cuda", generator=g)).to(TYPES[r])[1:]
+    big_h, H = place(torch.zeros(rows, O, device="cuda", dtype=TYPES[r]), 7)
+    nb = O if kind == "mxf8" else O // 2
+    big_q, D = place(torch.zeros(rows, nb, dtype=torch.uint8, device="cuda"), 77)
+    big_s, S = place(torch.zeros(rows, -(-O // 32), dtype=torch.uint8, device="cuda"), 66)
+    out = vm.MXDense(D.view(torch.float8_e4m3fn) if kind == "mxf8" else D, S, cols=O)
+    Q, h, inv = vm.add_rms_norm(X, w, residual=R, kind=KINDS[kind], out=out, residual_out=H)
+    assert Q is out and h is H
+    s = (X.float() + R.float()).to(TYPES[r])
+    assert torch.equal(H, s)
+    check_norm(out, inv, s, w, 1e-6, kind)
+    dY = place(torch.randn(rows, O, device="cuda", generator=g).to(TYPES[x]), 7)[1]
+    big_d, dR = place(torch.randn(rows, O, device="cuda", generator=g).to(TYPES[r]), 7)
+    dx, dw, size, dw_size = ref.norm_backward(np64(dY), np64(w), np64(H), np64(inv), np64(dR))
+    got, got_w = vm.add_rms_norm_backward(dY, w, H, inv, d_residual=dR, out=dR)  # in place
+    half = torch.finfo(TYPES[r]).eps / 2
+    assert got is dR and np.all(np.abs(np64(got) - dx) <= half * np.abs(dx) + 8 * U * size * (1 + half) + 2.0 ** -24)
+    assert np.all(np.abs(np64(got_w) - dw) <= (rows + 4) * U * dw_size)
+    for big, view, fill in ((big_h, H, 7), (big_q, D, 77), (big_s, S, 66), (big_d, dR, 7)):
+        view.fill_(fill)
+        assert bool((big == fill).all())
+
+
+def test_norm_refusals_with_tensors(cuda):
+    X, w = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    half = X.half()
+    Q, h, inv = vm.add_rms_norm(X, w, residual=X)
+    for call in (lambda: vm.add_rms_norm(X, w[:63]), lambda: vm.add_rms_norm(X, w.cpu()), lambda: vm.add_rms_norm(X, w.double()),
+                 lambda: vm.add_rms_norm(half, w, residual=X), lambda: vm.add_rms_norm(X, w, residual=X[:3]),
+                 lambda: vm.add_rms_norm(X, w, residual=half, residual_out=X), lambda: vm.add_rms_norm(X, w, eps=-1.0),
+                 lambda: vm.add_rms_norm(X, w, kind=vm.F16), lambda: vm.add_rms_norm(X, w, kind=vm.MXF4, out=Q),
+                 lambda: vm.add_rms_norm(X.t(), w), lambda: vm.add_rms_norm(X[0], w), lambda: vm.add_rms_norm(X.expand(2, 4, 64)[0].double(), w),
+                 lambda: vm.add_rms_norm(X[:1].expand(4, 64), w), lambda: vm.add_rms_norm(X, None),
+                 lambda: vm.add_rms_norm_backward(X, w, h, inv.half()), lambda: vm.add_rms_norm_backward(half, w, h, inv),
+                 lambda: vm.add_rms_norm_backward(X, w, h, inv[:3]), lambda: vm.add_rms_norm_backward(X, w, h, inv, out=half),
+                 lambda: vm.mx_quantize(X, 9), lambda: vm.mx_quantize(X.long()), lambda: vm.mx_dequantize(Q, dtype=torch.float16, out=X),
+                 lambda: vm.mx_dequantize(Q, out=X[:, :32])):
+        with pytest.raises((vm.VcsrmcError, RuntimeError)):
+            call()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("O", [100, 128, 1000, 16392])
+def test_norm_in_place_on_its_first_operand(cuda, O):
+    """residual_out is X, and dX is dY: the same bits as in tensors of their own."""
+    g = torch.Generator("cuda").manual_seed(O)
+    X, R, dY = (torch.randn(70, O, device="cuda", generator=g).half() for _ in range(3))
+    w = torch.randn(O, device="cuda", generator=g)
+    for residual in (R, None):
+        Q, h, inv = vm.add_rms_norm(X, w, residual=residual)
+        h = h.clone()
+        place = X.clone()
+        Q2, h2, inv2 = vm.add_rms_norm(place, w, residual=residual, residual_out=place)
+        assert h2 is place and torch.equal(place, h) and torch.equal(inv2, inv)
+        assert all(np.array_equal(a, b) for a, b in zip(codes_of(Q), codes_of(Q2)))
+        dx, dw = vm.add_rms_norm_backward(dY, w, h, inv, d_residual=residual)
+        place = dY.clone()
+        dx2, dw2 = vm.add_rms_norm_backward(place, w, h, inv, d_residual=residual, out=place)
+        assert dx2 is place and torch.equal(dx2, dx) and torch.equal(dw2, dw)
+
+
+@pytest.mark.parametrize("rows,O", [(540_000_000, 1), (17_000_000, 136)])
+def test_many_rows(cuda, rows, O):
+    """More than 2^31 values, and more groups of them than a launch numbers: the first rows, the last, and those around each border."""
+    kind, nb = ("mxf4", (O + 1) // 2) if O == 1 else ("mxf8", O)
+    X = torch.zeros(rows, O, dtype=torch.float16, device="cuda")
+    picks = sorted({r for b in (0, (1 << 31) // O, (1 << 31) // (2 * O), 0x7f000000 // 4, 0x7f000000 // (16 if O == 1 else 32), rows) for r in range(b - 3, b + 3)
+                    if 0 <= r < rows})
+    at = torch.tensor(picks, device="cuda")
+    X[at] = torch.randn(len(picks), O, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).half()
+    x = np64(X[at])
+    data = torch.full((rows, nb), 77, dtype=torch.uint8, device="cuda")
+    scale = torch.full((rows, -(-O // 32)), 66, dtype=torch.uint8, device="cuda")
+    out = vm.MXDense(data.view(torch.float8_e4m3fn) if kind == "mxf8" else data, scale, cols=O)
+    want_codes, want_scales = ref.quantize(x.astype(np.float32), kind)
+
+    def check_rest():
+        used = torch.zeros(rows, dtype=torch.bool, device="cuda")
+        used[at] = True
+        assert int((data != 0).any(1).logical_and(~used).sum()) == 0 and int((scale != 0).any(1).logical_and(~used).sum()) == 0
+
+    vm.mx_quantize(X, KINDS[kind], out=out)
+    got = data[at].cpu().numpy() if kind == "mxf8" else ref.unpack(data[at].cpu().numpy(), O)
+    assert np.array_equal(got, want_codes) and np.array_equal(scale[at].cpu().numpy(), want_scales)
+    check_rest()
+    Y = torch.full((rows, O), 9.0, dtype=torch.float16, device="cuda")
+    vm.mx_dequantize(out, out=Y)
+    assert np.array_equal(np64(Y[at]), ref.values(want_codes, want_scales, kind).astype(np.float16).astype(np.float64))
+    assert int((Y != 0).any(1).sum()) <= len(picks)
+    # the norm of the same rows; rows of zeros have zeros and 1 / sqrt(eps)
+    w = torch.full((O,), 1.5, device="cuda")
+    _, h, inv = vm.add_rms_norm(X, w, kind=KINDS[kind], out=out, eps=1e-4)
+    check_norm(vm.MXDense(out.data.view(torch.uint8)[at].view(out.data.dtype), scale[at], cols=O), inv[at], X[at], w, 1e-4, kind)
+    check_rest()
+    dx, dw, size, dw_size = ref.norm_backward(x, np64(w), x, np64(inv[at]), None)
+    got, got_w = vm.add_rms_norm_backward(X, w, X, inv, out=Y)
+    assert np.all(np.abs(np64(got[at]) - dx) <= 2.0 ** -11 * np.abs(dx) + 8 * U * size * (1 + 2.0 ** -11) + 2.0 ** -24)
+    assert np.all(np.abs(np64(got_w) - dw) <= (len(picks) + 4) * U * dw_size)  # terms of zero round nothing
+    assert int((got != 0).any(1).sum()) <= len(picks)
