@@ -193,7 +193,7 @@ def test_product_shapes(cuda, kind, M, N, density, unit, built):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("O,pitch,shift", [(128, 256, 0), (128, 160, 16), (128, 136, 8), (128, 132, 4), (128, 131, 0), (96, 129, 1), (64, 99, 2), (100, 112, 0),
+@pytest.mark.parametrize("O,pitch,shift", [(128, 256, 0), (128, 160, 16), (128, 136, 8), (128, 132, 4), (128, 131, 0), (96, 129, 1), (64, 99, 2), (100, 112, 0), (100, 104, 8), (99, 120, 24), (136, 168, 8),
                                            (45, 61, 3)])
 def test_product_strides(cuda, kind, O, pitch, shift):
     """B in a larger buffer at any alignment, its scales too; C in a larger buffer whose other columns and rows stay."""

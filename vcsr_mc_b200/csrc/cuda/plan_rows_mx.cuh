@@ -514,30 +514,49 @@ cudaError_t launch(Args a, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-// Wide: the form for aligned loads of a whole lane, Narrow for word by word, which takes more registers per column.
-template <bool k4, class Wide, class Narrow, typename VT>
-cudaError_t launch_lanes(const Args& a, cudaStream_t st) {
-    const uintptr_t q = reinterpret_cast<uintptr_t>(a.B.q);
-    const int64_t full = k4 ? Wide::kCols / 2 : Wide::kCols, row_bytes = k4 ? (int64_t(a.O) + 1) / 2 : a.O;
-    if (q % full == 0 && a.B.ldq % full == 0) {
-        if (a.O % Wide::kCols == 0) return launch<k4, Wide, Access::kWhole, VT>(a, st);
-        if (a.B.ldq >= (row_bytes + full - 1) / full * full) return launch<k4, Wide, Access::kPadded, VT>(a, st);
-    }
-    if (q % 4 == 0 && a.B.ldq % 4 == 0) return launch<k4, Narrow, Access::kWords, VT>(a, st);
-    return launch<k4, Narrow, Access::kBytes, VT>(a, st);
+// One load for a lane's columns, where every row is aligned to it and the operand's rows are whole loads or padded to them.
+// True where that holds; the launch's result is in e.
+template <bool k4, class L, typename VT>
+bool launch_whole(const Args& a, cudaStream_t st, cudaError_t& e) {
+    const int64_t full = k4 ? L::kCols / 2 : L::kCols, row_bytes = k4 ? (int64_t(a.O) + 1) / 2 : a.O;
+    if (reinterpret_cast<uintptr_t>(a.B.q) % uintptr_t(full) || a.B.ldq % full) return false;
+    if (a.O % L::kCols == 0) e = launch<k4, L, Access::kWhole, VT>(a, st);
+    else if (a.B.ldq >= (row_bytes + full - 1) / full * full) e = launch<k4, L, Access::kPadded, VT>(a, st);
+    else return false;
+    return true;
+}
+
+// Words, Bytes: the forms for rows that are read word by word, aligned to words or not.
+template <bool k4, class Words, class Bytes, typename VT>
+cudaError_t launch_words(const Args& a, cudaStream_t st) {
+    if (reinterpret_cast<uintptr_t>(a.B.q) % 4 == 0 && a.B.ldq % 4 == 0) return launch<k4, Words, Access::kWords, VT>(a, st);
+    return launch<k4, Bytes, Access::kBytes, VT>(a, st);
 }
 
 template <bool k4, typename VT>
 cudaError_t product_columns(const Args& a, cudaStream_t st) {
     // Columns per lane and entries in flight as measured on 262144 rows of 16 entries, O = 32: 4 lanes of 8 columns 60
     // (E2M1) and 60 us (E4M3, four in flight; eight: 71), 2 lanes of 16: 74 and 75; O = 64: 8 lanes of 8 columns 67,
-    // 4 of 16 85 us; O = 128: 16 lanes of 8 columns 96, as 8 of 16, but 468 against 409 us on the stencil. Word by
-    // word, O = 300 in 4 bits: 381 against 438 us; O = 100, fp32 A: 129 against 149 us; O = 101 in 8 bits, fp16 A:
-    // 195 against 180 us.
-    if (a.O <= 32) return launch_lanes<k4, Lanes<4, 8, k4 ? 8 : 4>, Lanes<4, 8, k4 ? 8 : 4>, VT>(a, st);
-    if (a.O <= 64) return launch_lanes<k4, Lanes<8, 8, 8>, Lanes<8, 8, 8>, VT>(a, st);
-    using Narrow = typename std::conditional<k4 || sizeof(VT) == 4, Lanes<16, 8, 8>, Lanes<8, 16, 8>>::type;
-    return launch_lanes<k4, Lanes<8, 16, 8>, Narrow, VT>(a, st);
+    // 4 of 16 85 us; O = 128: 16 lanes of 8 columns 96, as 8 of 16, but 468 against 409 us on the stencil.
+    cudaError_t e;
+    if (a.O <= 32) {
+        using L = Lanes<4, 8, k4 ? 8 : 4>;
+        return launch_whole<k4, L, VT>(a, st, e) ? e : launch_words<k4, L, L, VT>(a, st);
+    }
+    if (a.O <= 64) {
+        using L = Lanes<8, 8, 8>;
+        return launch_whole<k4, L, VT>(a, st, e) ? e : launch_words<k4, L, L, VT>(a, st);
+    }
+    using Wide = Lanes<8, 16, 8>;
+    using Narrow = Lanes<16, 8, 8>;
+    if (launch_whole<k4, Wide, VT>(a, st, e)) return e;
+    // E4M3 rows at multiples of 8 bytes: 8 columns in one load, O = 120, 104 against 138 us word by word (stencil 482
+    // against 635, R-MAT 448 against 618; eight entries in flight: 109, 509, 457)
+    if constexpr (!k4)
+        if (launch_whole<k4, Lanes<16, 8, 4>, VT>(a, st, e)) return e;
+    // Word by word, 8 columns against 16: O = 300 in 4 bits 381 against 438 us; O = 100 in 8 bits 121 against 134 us,
+    // fp32 A 129 against 149 us; but O = 101 in 8 bits, fp16 A, 195 against 180 us.
+    return launch_words<k4, Narrow, typename std::conditional<k4 || sizeof(VT) == 4, Narrow, Wide>::type, VT>(a, st);
 }
 
 // One pair of element and A value types; each pair is a translation unit. Up to 64 columns behind the last whole slab
