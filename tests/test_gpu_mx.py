@@ -725,3 +725,39 @@ def test_many_rows(cuda, rows, O):
     assert np.all(np.abs(np64(got[at]) - dx) <= 2.0 ** -11 * np.abs(dx) + 8 * U * size * (1 + 2.0 ** -11) + 2.0 ** -24)
     assert np.all(np.abs(np64(got_w) - dw) <= (len(picks) + 4) * U * dw_size)  # terms of zero round nothing
     assert int((got != 0).any(1).sum()) <= len(picks)
+
+
+def test_default_stream_by_its_handle(cuda):
+    """stream=0, the default stream's handle as torch gives it: every call runs behind what that stream already holds, while another stream
+    is the current one."""
+    from vcsr_mc_b200.api import _stream_guard
+    device = torch.device("cuda", torch.cuda.current_device())
+    default = torch.cuda.default_stream(device)
+    for given in (0, 1, default.cuda_stream, default):
+        with _stream_guard(given, device):
+            assert torch.cuda.current_stream() == default
+    M, O = 64, 40
+    csr = sparse(M, M, 0.3, 2)
+    dV = handle(M, M, *csr, False)
+    g = torch.Generator("cuda").manual_seed(5)
+    new, w = torch.randn(M, O, device="cuda", generator=g), torch.ones(O, device="cuda")
+
+    def calls(X, Y, C, h, inv, stream):
+        Q = vm.mx_quantize(X, vm.MXF8, stream=stream)
+        vm.mx_dequantize(Q, out=Y, stream=stream)
+        vm.spmm(dV, Q, C, stream=stream)
+        N, H, I = vm.add_rms_norm(C, w, residual=X, stream=stream)
+        return (Q.data, Q.scale, Y, C, N.data, N.scale, H, I) + tuple(vm.add_rms_norm_backward(X, w, h, inv, stream=stream))
+
+    inv = 1 / torch.sqrt(new.square().mean(1) + 1e-6)
+    want = calls(new, torch.empty_like(new), torch.empty(M, O, device="cuda"), new, inv, None)
+    X, h = torch.zeros_like(new), torch.zeros_like(new)
+    Y, C, side = torch.empty_like(new), torch.empty(M, O, device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(40_000_000)  # about 20 ms, before X is there
+    X.copy_(new)
+    h.copy_(new)
+    with torch.cuda.stream(side):
+        got = calls(X, Y, C, h, inv, default.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))

@@ -124,3 +124,18 @@ def test_mx_matrix_is_what_was_checked():
                         ("kind", vm.MXF8), ("shape", (9, 9)), ("anything", 1)):
         with pytest.raises(AttributeError):
             setattr(Q, name, value)
+
+
+@pytest.mark.parametrize("raw,want", [(0, "default"), (1, "default"), (2, 2), (0x7F0012345678, 0x7F0012345678)])
+def test_raw_stream_handles(monkeypatch, raw, want):
+    """A raw handle names the stream that CUDA means by it: 0 and 1 are the default stream (which torch itself gives as 0; an external
+    stream made from it would be another one), any other is taken as it is."""
+    from types import SimpleNamespace
+    from vcsr_mc_b200 import api
+    device = torch.device("cuda:0")
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda d: SimpleNamespace(which="default", device=d))
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda raw, device: SimpleNamespace(which=raw, device=device))
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: s)
+    for given in (raw, SimpleNamespace(cuda_stream=raw)):
+        guard = api._stream_guard(given, device)
+        assert guard.which == want and guard.device == device

@@ -430,7 +430,8 @@ def _stream_guard(stream, device):
         raise _invalid("microscaled operators run on CUDA tensors")
     if not isinstance(stream, torch.cuda.Stream):
         raw = int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
-        stream = torch.cuda.ExternalStream(raw, device=device)
+        # 0 and 1 are the default stream, as torch and CUDA give it; torch makes another stream of an external 0
+        stream = torch.cuda.default_stream(device) if raw in (0, 1) else torch.cuda.ExternalStream(raw, device=device)
     if stream.device != device:
         raise _invalid(f"the stream must be on {device}, with the tensors")
     return torch.cuda.stream(stream)
