@@ -761,3 +761,65 @@ def test_default_stream_by_its_handle(cuda):
         got = calls(X, Y, C, h, inv, default.cuda_stream)
     torch.cuda.synchronize()
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+
+
+def scale_rows(scales, pitch, fill):
+    """Scales on rows `pitch` bytes apart, in an array that ends with the last row's last scale; the bytes between rows hold `fill`."""
+    N, blocks = scales.shape
+    flat = torch.from_numpy(np.resize(np.asarray(fill, np.uint8), (N - 1) * pitch + blocks)).cuda()
+    view = torch.as_strided(flat, (N, blocks), (pitch, 1))
+    view.copy_(torch.from_numpy(scales))
+    return view
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("O,first", [(65, None), (72, None), (96, None), (200, None), (224, None), (256, 70)])
+def test_product_padded_scales(cuda, kind, O, first):
+    """Scale rows of whole words whose slab has three blocks: whatever stands in the fourth byte (or the blocks of columns that are not asked
+    for), the results are the same bits. The last row is an entry, and the array ends with its last scale."""
+    M, N = 70, 50
+    csr = sparse(M, N, 0.3, O, long_row=4)
+    codes, scales = features(N, O, O, kind)
+    blocks = scales.shape[1]
+    want, size, n = ref.product(*csr, ref.values(codes, scales, kind)[:, :first])
+    data = to_mx(codes, scales, kind, pitch=(codes.shape[1] + 15) // 16 * 16 if kind == "mxf8" else None).data
+    rng = np.random.default_rng(O)
+    for fp32 in (False, True):
+        dV, seen = handle(M, N, *csr, fp32, rows_unit_nnz=16), []
+        for fill in (0, 255, 1, rng.integers(0, 256, N * 8)):
+            held = scales.copy()
+            if first:
+                held[:, 3:] = np.resize(fill, (N, blocks - 3))
+            C = torch.empty(M, first or O, device="cuda")
+            vm.spmm(dV, vm.MXDense(data, scale_rows(held, (blocks + 3) // 4 * 4, fill), cols=O), C, O=first)
+            assert np.all(np.abs(np64(C) - want) <= (n + 4) * U * size)
+            seen.append(C)
+        assert all(torch.equal(C, seen[0]) for C in seen)
+
+
+def test_product_time_does_not_follow_padding(cuda):
+    """The bytes behind a row's last scale do not choose the form of the product: the least of ten times is the same within a few percent
+    (the fp32 form, which a 255 there once chose, takes 15 % longer here)."""
+    M, O = 1 << 18, 96
+    g = torch.Generator("cuda").manual_seed(1)
+    key = torch.unique(torch.randint(0, M * M, (16 * M,), device="cuda", generator=g))
+    rp = torch.zeros(M + 1, dtype=torch.int32, device="cuda")
+    rp[1:] = torch.cumsum(torch.bincount(key // M, minlength=M), 0)
+    val = (torch.rand(key.numel(), device="cuda", generator=g) * 2 - 1).half().float()
+    dV = vm.build_vcsr_mc_device(rp, (key % M).int(), val, M, M, segw=32, plans=[vm.PLAN_ROWS])
+    Q = vm.mx_quantize(torch.randn(M, O, device="cuda", generator=g), vm.MXF8)
+    rows = torch.as_strided(Q.scale.view(torch.uint8), (M, 4), (4, 1))
+    assert Q.scale.stride(0) == 4
+    C, best = torch.empty(M, O, device="cuda"), {0: 1e9, 255: 1e9}
+    for _ in range(10):
+        for fill in best:
+            rows[:, 3] = fill
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda._sleep(400_000)
+            a.record()
+            for _ in range(6):
+                vm.spmm(dV, Q, C)
+            b.record()
+            torch.cuda.synchronize()
+            best[fill] = min(best[fill], a.elapsed_time(b))
+    assert best[255] < 1.07 * best[0], best

@@ -261,6 +261,11 @@ __global__ void __launch_bounds__(kWarps * 32) rows_mx_kernel(Args P) {
     }
     const uint8_t* s_base = P.B.s + slab / kMxBlock;
     const int blocks = min(kBlocks, (exist + kMxBlock - 1) / kMxBlock);
+    // What stands behind a row's last scale is nobody's, and no part of the choice between the fp16 and the fp32 form
+    // below. Cut at the scales' use and not at their load, which the warp would wait for (R-MAT 420 against 400 us), and
+    // not in the form that reads elements byte by byte, whose registers it does not fit (O = 101: 203 against 181 us).
+    constexpr bool kCut = kBlocks == 4 && kAccess != Access::kBytes;
+    const uint32_t existing = 0xffffffffu >> (8 * (4 - blocks));
     const uint32_t ldq = uint32_t(P.B.ldq), lds = uint32_t(P.B.lds);
 
     // the unit's entries (positions below count from its first) and rows
@@ -329,7 +334,9 @@ __global__ void __launch_bounds__(kWarps * 32) rows_mx_kernel(Args P) {
         if (c < 0) c = __ldg(P.hot_cols + ~c);  // a ranked hot column
         const uint8_t* s = s_base + uint64_t(uint32_t(c)) * lds;
         if constexpr (kBlocks == 1) return __ldg(s);
-        if (P.scale_words) {
+        // In one word where it ends with the slab's blocks or before the operand does (`kCut`: the rest of it is cut off
+        // when it is used), else byte by byte.
+        if (P.scale_words && (blocks == kBlocks || (kCut && c != P.N - 1))) {
             if constexpr (kBlocks == 4) return __ldg(reinterpret_cast<const uint32_t*>(s));
             else return __ldg(reinterpret_cast<const unsigned short*>(s));
         }
@@ -356,11 +363,12 @@ __global__ void __launch_bounds__(kWarps * 32) rows_mx_kernel(Args P) {
         float a[kPer][kBlocks];
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            const float2 s01 = scale_pair(s_now[k], 0);
+            const uint32_t codes = kAcc16 && kCut ? s_now[k] & existing : s_now[k];
+            const float2 s01 = scale_pair(codes, 0);
             a[k][0] = mul_ftz(v_now[k], s01.x);
             if constexpr (kBlocks > 1) a[k][1] = mul_ftz(v_now[k], s01.y);
             if constexpr (kBlocks > 2) {
-                const float2 s23 = scale_pair(s_now[k], 1);
+                const float2 s23 = scale_pair(codes, 1);
                 a[k][2] = mul_ftz(v_now[k], s23.x);
                 a[k][3] = mul_ftz(v_now[k], s23.y);
             }
