@@ -82,10 +82,7 @@ int64_t rows_mx_pitch(int O) { return (int64_t(O) + 3) / 4 * 4; }
 
 cudaError_t spmm_rows_mx(const RowPlanView& P, const MxView& B, int O, float* C, int64_t ldc, bool accumulate,
                          float* partial, cudaStream_t st) {
-    if (P.n_units == 0) {
-        if (!accumulate && P.M > 0) return cudaMemset2DAsync(C, size_t(ldc) * 4, 0, size_t(O) * 4, size_t(P.M), st);
-        return cudaSuccess;
-    }
+    if (P.n_units == 0) return cudaSuccess;  // no rows: every row, empty ones too, is a unit's
     rows_mx::Args a;
     a.units = P.units;
     a.n_units = P.n_units;

@@ -522,15 +522,13 @@ cudaError_t launch(Args a, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-// One load for a lane's columns, where every row is aligned to it and the operand's rows are whole loads or padded to them.
-// True where that holds; the launch's result is in e.
+// One load for a lane's columns, where every row is aligned to it; the row stride, a multiple of it, then pads a row that
+// ends inside a load. True where that holds; the launch's result is in e.
 template <bool k4, class L, typename VT>
 bool launch_whole(const Args& a, cudaStream_t st, cudaError_t& e) {
-    const int64_t full = k4 ? L::kCols / 2 : L::kCols, row_bytes = k4 ? (int64_t(a.O) + 1) / 2 : a.O;
+    const int64_t full = k4 ? L::kCols / 2 : L::kCols;
     if (reinterpret_cast<uintptr_t>(a.B.q) % uintptr_t(full) || a.B.ldq % full) return false;
-    if (a.O % L::kCols == 0) e = launch<k4, L, Access::kWhole, VT>(a, st);
-    else if (a.B.ldq >= (row_bytes + full - 1) / full * full) e = launch<k4, L, Access::kPadded, VT>(a, st);
-    else return false;
+    e = a.O % L::kCols == 0 ? launch<k4, L, Access::kWhole, VT>(a, st) : launch<k4, L, Access::kPadded, VT>(a, st);
     return true;
 }
 
