@@ -823,3 +823,146 @@ def test_product_time_does_not_follow_padding(cuda):
             torch.cuda.synchronize()
             best[fill] = min(best[fill], a.elapsed_time(b))
     assert best[255] < 1.07 * best[0], best
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("O,pitch", [(24, 32), (64, 64), (128, 128), (120, 120), (100, 100), (101, 101)])
+def test_product_changes_form_within_a_unit(cuda, kind, O, pitch):
+    """FP16 format: batches of eight entries whose scales fit the fp16 form of a unit, then do not, then do again, in rows that end with a batch,
+    inside one or after several. Rows of small values stand between rows of large ones, so a factor left behind by a change shows in them."""
+    lens = [8, 8, 8, 8, 8, 5, 3, 0, 8, 13, 11, 0, 40, 24, 1, 1, 6, 60, 4, 8, 8]
+    codes_by_place = [[127, 190, 127, 40, 127], [127, 127, 180, 127, 90], [60, 127, 127, 200, 127], [127, 100, 150, 127, 127]]
+    M, N = 6 * len(lens), 6 * sum(lens)  # every entry its own row of B
+    rp = np.concatenate([[0], np.cumsum(np.tile(lens, 6))]).astype(np.int32)
+    rng = np.random.default_rng(O)
+    col, val = np.arange(N, dtype=np.int32), (rng.uniform(0.5, 1, N) * rng.choice([-1, 1], N)).astype(np.float16).astype(np.float32)
+    codes, scales = features(N, O, 3, kind)
+    # the scale of entry e in block b: by its place in runs of eight, another sequence for every block and sixth of the matrix
+    e = np.arange(N)
+    sixth = e // sum(lens)
+    for b in range(scales.shape[1]):
+        seq = np.array(codes_by_place)[(b + sixth) % 4, (e % sum(lens)) // 8 % 5]
+        scales[:, b] = np.where(sixth == 5, 127 + e % 3, seq)  # the last sixth never leaves the fp16 form
+    Q = to_mx(codes, scales, kind, pitch=pitch if kind == "mxf8" else (pitch + 1) // 2)
+    for unit in (16, 64, 256):
+        dV = handle(M, N, rp, col, val, False, rows_unit_nnz=unit)
+        C = check_product(dV, (rp, col, val), codes, scales, kind, Q=Q)
+        start = C * 0.5
+        check_product(dV, (rp, col, val), codes, scales, kind, Q=Q, start=start)
+
+
+@pytest.fixture(scope="module")
+def many_split_rows():
+    """20000 rows, most of 65 to 200 entries: more than 8192 rows that are split into chunks of 16, and as many units."""
+    M, N = 20000, 3000
+    rng = np.random.default_rng(7)
+    lens = rng.integers(65, 201, M)
+    lens[::50], lens[1::50], lens[2::50] = 0, 3, 16
+    rp = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    first, step = rng.integers(0, N, M), rng.integers(1, 14, M)  # N / 14 > 200: a row's columns are distinct
+    at = np.arange(rp[-1]) - np.repeat(rp[:-1], lens)
+    row = np.repeat(np.arange(M), lens)
+    col = (np.repeat(first, lens) + at * np.repeat(step, lens)) % N
+    order = np.lexsort((col, row))
+    col = col[order].astype(np.int32)
+    val = rng.uniform(-1, 1, len(col)).astype(np.float16).astype(np.float32)
+    return M, N, rp, col, val
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("fp32", [False, True])
+@pytest.mark.parametrize("O", [129, 132, 160, 192, 300])
+def test_product_slabs_and_chunks(cuda, many_split_rows, kind, fp32, O):
+    """Columns behind the last whole slab in a launch of their own, and the chunks of many split rows added up behind both: stored and
+    accumulated, in contiguous and odd places."""
+    M, N, rp, col, val = many_split_rows
+    dV = handle(M, N, rp, col, val, fp32, rows_unit_nnz=16)
+    codes, scales = features(N, O, O, kind)
+    A = torch.zeros(M, N, dtype=torch.float64, device="cuda")
+    A[torch.from_numpy(np.repeat(np.arange(M), np.diff(rp))).cuda(), torch.from_numpy(col).long().cuda()] = torch.from_numpy(val).double().cuda()
+    B = torch.from_numpy(ref.values(codes, scales, kind)).cuda()
+    want, size, n = A @ B, A.abs() @ B.abs(), int(np.diff(rp).max())
+    slack = 1 + 2.0 ** -40  # of the 64-bit products
+    nb = O if kind == "mxf8" else (O + 1) // 2
+    for pitch in (nb, (nb + 15) // 16 * 16, nb + 3):
+        Q = to_mx(codes, scales, kind, pitch=pitch)
+        first = None
+        for off, ldc in ((0, O), (1, O + 3)):
+            big = torch.full((M + 2, ldc), 3.5, device="cuda")
+            C = big[1:M + 1, off:off + O]
+            vm.spmm(dV, Q, C)
+            assert bool(((C.double() - want).abs() <= (n + 4) * U * size * slack).all())
+            assert first is None or torch.equal(C, first)
+            first = C.clone()
+            start = torch.randn(M, O, device="cuda", generator=torch.Generator("cuda").manual_seed(O))
+            C.copy_(start)
+            vm.spmm(dV, Q, C, accumulate=True)
+            bound = (n + 4) * U * (size + start.double().abs()) * slack
+            assert bool(((C.double() - want - start.double()).abs() <= bound).all())
+            C.fill_(3.5)
+            assert bool((big == 3.5).all())
+
+
+@pytest.mark.parametrize("x,r", COMBOS)
+@pytest.mark.parametrize("rows,O", [(700, 264), (700, 4097), (700, 5000), (700, 8192), (700, 8193), (650, 16392)])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_norm_backward_more_rows_than_blocks(cuda, x, r, rows, O, aligned):
+    """Wide rows, several to a block (two blocks per SM at most): the next row's loads, the weight's gradient over a block's rows. A row's sum
+    has at most O / 256 terms in turn in a thread and ten steps over threads, and the other terms 8 roundings."""
+    g = torch.Generator("cuda").manual_seed(rows + O)
+
+    def make(t):
+        if aligned:
+            return torch.randn(rows, O, device="cuda", generator=g).to(TYPES[t])
+        return torch.randn(rows, O + 5, device="cuda", generator=g).to(TYPES[t])[:, 3:3 + O]
+
+    dY, dR, h = make(x), make(r), make(r)
+    w = (1 + 0.2 * torch.randn(O, device="cuda", generator=g)).to(TYPES[r])
+    inv = (1 / torch.sqrt(h.double().square().mean(1) + 1e-5)).float()
+    n, gw = h.double() * inv.double()[:, None], dY.double() * w.double()
+    through = inv.double()[:, None] * n
+    dw, dw_size = (dY.double() * n).sum(0), (dY.double() * n).abs().sum(0)
+    half, roundings = torch.finfo(TYPES[r]).eps / 2, 8 + O / 256 + 10
+    results = []
+    for d_residual in (dR, None):
+        base = 0.0 if d_residual is None else d_residual.double()
+        dx = base + inv.double()[:, None] * gw - through * (gw * n).mean(1, keepdim=True)
+        size = (base if d_residual is None else base.abs()) + (inv.double()[:, None] * gw).abs() + through.abs() * (gw * n).abs().mean(1, keepdim=True)
+        got, got_w = vm.add_rms_norm_backward(dY, w, h, inv, d_residual=d_residual)
+        tiny = float(torch.finfo(TYPES[r]).smallest_normal) * float(torch.finfo(TYPES[r]).eps)
+        assert bool(((got.double() - dx).abs() <= half * dx.abs() + roundings * U * size * (1 + half) + tiny).all())
+        assert bool(((got_w.double() - dw).abs() <= (rows + 4) * U * dw_size).all())
+        results.append((got, got_w))
+    place = dR.clone() if aligned else torch.cat([dR, dR[:, :5]], 1)[:, :O].copy_(dR)
+    out, out_w = vm.add_rms_norm_backward(dY, w, h, inv, d_residual=place, out=place)
+    assert out is place and torch.equal(place, results[0][0]) and torch.equal(out_w, results[0][1])
+    if x == r:  # in place on dY
+        out, out_w = vm.add_rms_norm_backward(dY, w, h, inv, out=dY)
+        assert out is dY and torch.equal(dY, results[1][0]) and torch.equal(out_w, results[1][1])
+
+
+def test_refusals_are_argument_errors(cuda):
+    """What is refused is refused as an invalid argument, before anything runs: no other error counts, and the next call is right."""
+    X, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    half = X.half()
+    Q, h, inv = vm.add_rms_norm(X, w, residual=X)
+    other = vm.MXDense.empty(4, 32)
+    for call in (lambda: vm.add_rms_norm(X, w[:63]), lambda: vm.add_rms_norm(X, w.cpu()), lambda: vm.add_rms_norm(X, w.double()),
+                 lambda: vm.add_rms_norm(half, w, residual=X), lambda: vm.add_rms_norm(X, w, residual=X[:3]),
+                 lambda: vm.add_rms_norm(X, w, residual=half, residual_out=X), lambda: vm.add_rms_norm(X, w, eps=-1.0),
+                 lambda: vm.add_rms_norm(X, w, kind=vm.F16), lambda: vm.add_rms_norm(X, w, kind=vm.MXF4, out=Q),
+                 lambda: vm.add_rms_norm(X.t(), w), lambda: vm.add_rms_norm(X[0], w), lambda: vm.add_rms_norm(X[:1].expand(4, 64), w),
+                 lambda: vm.add_rms_norm(X, None), lambda: vm.add_rms_norm(X, w, out=other), lambda: vm.add_rms_norm(X, w, eps=float("inf")),
+                 lambda: vm.add_rms_norm(X, torch.ones(128, device="cuda")[::2]), lambda: vm.add_rms_norm(X[:, :0], w[:0]),
+                 lambda: vm.add_rms_norm_backward(X, w, h, inv.half()), lambda: vm.add_rms_norm_backward(half, w, h, inv),
+                 lambda: vm.add_rms_norm_backward(X, w, h, inv[:3]), lambda: vm.add_rms_norm_backward(X, w, h, inv, out=half),
+                 lambda: vm.add_rms_norm_backward(X, w, h, None), lambda: vm.add_rms_norm_backward(X, w, h, inv, d_residual=half),
+                 lambda: vm.mx_quantize(X, 9), lambda: vm.mx_quantize(X.long()), lambda: vm.mx_quantize(X[:, :0]), lambda: vm.mx_quantize(X, out=other),
+                 lambda: vm.mx_dequantize(Q, dtype=torch.float16, out=X), lambda: vm.mx_dequantize(Q, out=X[:, :32]),
+                 lambda: vm.mx_dequantize(Q, out=X.double()), lambda: vm.mx_dequantize(Q, out=X.cpu())):
+        with pytest.raises(vm.VcsrmcError) as e:
+            call()
+        assert e.value.status == 1, str(e.value)  # VCSRMC_INVALID_ARG
+    torch.cuda.synchronize()
+    again = vm.add_rms_norm(X, w, residual=X)
+    assert torch.equal(again[0].data.view(torch.uint8), Q.data.view(torch.uint8)) and torch.equal(again[1], h) and torch.equal(again[2], inv)
