@@ -264,7 +264,8 @@ int vcsrmc_spmm_timed(const vcsrmc_device_format* d, const void* B, int b_dtype,
  * aligned to their element type; row strides are in elements for dense matrices and in bytes for
  * MX elements (ldq) and scales (lds). O is in [1, 2^30] (products: [1, 8388480]). Outputs must not
  * overlap inputs unless a call says so; bytes between a row's end and its stride are left as they
- * are.
+ * are, and no result or choice depends on them. A product reads MX elements in whole aligned words of
+ * 4 bytes that hold at least one of a row's bytes: up to 3 bytes around the array, inside such a word.
  *
  * Q = MX(X): the scale of a block is the smallest power of two (at least 2^-127) under which its
  * largest magnitude fits the element type (448 for E4M3, 6 for E2M1), so nothing is clipped; elements
@@ -277,7 +278,10 @@ int vcsrmc_mx_dequantize(const void* Q, int q_dtype, int64_t ldq, const uint8_t*
                          int64_t rows, int32_t O, void* Y, int y_dtype, int64_t ldy, void* stream);
 /* C[M x O] (+)= A * B with an MX operand B (N rows): both formats, ROWS layout, fp32 sums whose order
  * is fixed (the same call gives the same bits). |a| * 2^(code - 127) of an entry and a block must be
- * finite, and counts as zero below fp32's normal range (2^-126), as in blocks of code 0. The workspace
+ * finite; where it is below fp32's normal range (2^-126) the entry counts as zero in that block. A block of
+ * code 0 counts as zero with every a, large ones too, whatever its elements: its scale, 2^-127, is itself below
+ * that range. (vcsrmc_mx_dequantize gives such a block's values, up to 448 * 2^-127 = 2^-118.2, as they are.)
+ * Adding to C may take values of C and sums below that range as zero. The workspace
  * (vcsrmc_spmm_mx_workspace bytes, 0 for a matrix without rows to split; 16-byte aligned) is the caller's,
  * so products of one handle may be in flight on several streams or in several graphs as long as each has
  * its own; it need not be initialised. */
@@ -289,7 +293,9 @@ int vcsrmc_spmm_mx(const vcsrmc_device_format* d, const void* Q, int q_dtype, in
  * inv_rms = 1 / sqrt(mean(s^2) + eps) of every row; Q = MX(s * inv_rms * weight). The residual (r_dtype)
  * has X's type, or X is fp32, as a product's C. residual NULL: s = X; residual_out or inv_rms NULL: not
  * stored. residual_out may be residual, or X where the types are the same, with the same stride. Values
- * are computed in fp32 from 64-bit square sums; the scale of a block is that of the 64-bit values. */
+ * are computed in fp32 (s * inv_rms, then * weight) from 64-bit square sums; the scale of a block is that
+ * of the 64-bit values, as long as inv_rms and s * inv_rms are normal numbers of fp32 (not so for rows whose
+ * root mean square is above 2^126, or with eps = 0 below 2^-128, where inv_rms is infinite). */
 int vcsrmc_add_rms_norm(const void* X, int x_dtype, int64_t ldx, const void* residual, int64_t ldr,
                         void* residual_out, int64_t ldo, int r_dtype, const void* weight, int w_dtype,
                         float eps, int64_t rows, int32_t O, int q_dtype, void* Q, int64_t ldq,

@@ -313,7 +313,8 @@ def _check_dense(B, C, O):
 def spmm(dV: DeviceVCSRMC, B, C, tileK: int = 128, accumulate: bool = False, stream=None, O: Optional[int] = None,
          plan: int = PLAN_AUTO):
     """C[:, :O] (+)= A * B[:, :O] on the GPU, asynchronous on `stream` (default: torch's current).
-    B: a float16 or float32 tensor, or an MXDense (ROWS plan; the same call gives the same bits)."""
+    B: a float16 or float32 tensor, or an MXDense (ROWS plan; the same call gives the same bits; blocks of scale code 0 count as zero).
+    stream: a torch stream or a raw handle (0: the default stream). Nothing is recorded for autograd."""
     if isinstance(B, MXDense):
         return _spmm_mx(dV, B, C, tileK, accumulate, stream, O, plan)
     O = int(B.shape[1]) if O is None else O
@@ -423,7 +424,7 @@ def _load_ops():
 
 
 def _stream_guard(stream, device):
-    """torch's guard that makes `stream` (a torch stream, or a raw handle) current on `device`, so that a call's launches and what it
+    """torch's guard that makes `stream` (a torch stream, or a raw handle; 0: the default stream) current on `device`, so that a call's launches and what it
     allocates belong to it."""
     import torch
     if device.type != "cuda":
@@ -487,7 +488,9 @@ def add_rms_norm(X, weight, residual=None, eps: float = 1e-6, kind: int = MXF8, 
                  stream=None):
     """(Q, residual_out, inv_rms): s = X + residual, rounded to the residual's type (residual_out); inv_rms = 1 / sqrt(mean(s^2) +
     eps) of every row (float32); Q = MX(s * inv_rms * weight). The residual has X's type, or X is float32 (a product's C). Without a
-    residual s is X, which is then returned in residual_out's place. residual_out may be the residual, or X of the same type (in place)."""
+    residual s is X, which is then returned in residual_out's place. residual_out may be the residual, or X of the same type (in place).
+    Nothing is recorded for autograd: new tensors do not require a gradient, whatever X does; add_rms_norm_backward is called by hand or from
+    a torch.autograd.Function of the caller's."""
     if stream is not None:
         with _stream_guard(stream, X.device):
             return add_rms_norm(X, weight, residual, eps, kind, out, residual_out)

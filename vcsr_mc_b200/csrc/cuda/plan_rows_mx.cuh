@@ -11,10 +11,11 @@
 // to a row of the workspace, and the chunks are added up in their order afterwards (join_chunks_kernel):
 // the result does not depend on the order in which the groups run.
 //
-// On a B200, O = 128 and E2M1: the 27-point stencil on 100^3 (26.5 M entries) takes 0.408 ms, bound by instructions (50
-// per warp for four entries, 30 of them decoding and multiplying, at 2.95 per clock and SM); the 2^20-row R-MAT
-// (16.1 M entries) 0.395 ms, 24.6 ps per entry, at the rate of random gathers (one of elements and one of scales per
-// entry). A and C move once; 739 and 706 MB would take 0.113 and 0.108 ms at the copy rate.
+// On a B200, O = 128 and E2M1, issue bounds both of the large cases: the 27-point stencil on 100^3 (26.5 M entries)
+// takes 0.411 ms, 51 instructions per warp for four entries, 30 of them decoding and multiplying, at 2.99 per clock
+// and SM; the 2^20-row R-MAT (16.2 M entries) 0.400 ms, 72 for four entries at 2.83, because a warp takes as many steps as
+// the longest of its groups (1.28 per entry, by its units). L2 is at 37 and 44 % of its throughput, DRAM at 24 and 23 %;
+// A and C move once, and 739 and 706 MB would take 0.113 and 0.108 ms at the copy rate.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -9,11 +9,14 @@
 //   dw = sum over rows of dy * n
 // The square sums are held in 64 bits: fp32 would overflow for |s| above 2^64, which bf16 and fp32 can
 // hold; the backward pass sums products of the normalised n, which cannot. Both passes read each input
-// once and write each output once (a row stays in registers up to 16384 columns forward and 8192 backward,
-// and is read a second time beyond), so HBM bounds them except for a few rows. On a B200 (copies run at 6.5 TB/s):
-// forward, 2^20 rows of 128, fp32 X and fp16 residual to E4M3, 190 us (6.4 TB/s); 20011 rows of 1009 (single
-// columns, bound by instructions), 43 us (4.2 TB/s); one row of 4096, 4.4 us. Backward, 32768 rows of 4096 in bf16,
-// 187 us (5.7 TB/s); 2^20 rows of 128, fp32 dY, fp16 else, 241 us (5.6 TB/s); 4096 rows of 128, 8.4 us.
+// once and write each output once (a row is held up to 16384 columns forward and 8192 backward, and is read a second
+// time beyond), so HBM bounds them except for a few rows, and for 4097 to 8192 columns backward: sixteen columns a
+// thread do not fit its 64 registers there (504 to 912 bytes of spills) and the row goes through local memory. On a B200
+// (copies run at 6.5 TB/s): forward, 2^20 rows of 128, fp32 X and fp16 residual to E4M3, 191 us (6.4 TB/s); 16384 rows of
+// 4096 in bf16, 90 us (5.2 TB/s); both up to 27 us more where one of the last rows has a block that rewrite_block takes;
+// 20011 rows of 1009 (single columns, bound by instructions), 43 us (4.2 TB/s); one row of 4096, 4.4 us.
+// Backward, 32768 rows of 4096 in bf16, 187 us (5.7 TB/s); 16384 rows of 8192, 526 us (2.0 TB/s), of 5001 (single
+// columns), 720 us; 2^20 rows of 128, fp32 dY, fp16 else, 244 us (5.5 TB/s); 4096 rows of 128, 8.4 us.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -42,8 +45,8 @@ struct Span {
     static constexpr int kRows = kL_ ? 256 / (kL_ ? kL_ : 1) : 1;  // rows in a block
     static constexpr int kW = kL_ ? kL_ : 32;      // threads whose groups are neighbours
     // forward blocks per SM that the registers are held to: with eight columns a thread, all of an SM's threads (2^20
-    // rows of 128: 191 against 202 us); with 16 in blocks of up to 512, three blocks (16384 rows of 4096: 110 against
-    // 115 us with four and 122 with two)
+    // rows of 128: 191 against 202 us); with 16 in blocks of up to 512, three blocks (16384 rows of 4096, with a late block
+    // that is written again: 110 against 115 us with four and 122 with two)
     static constexpr int kForwardBlocks = !kAny && kN == 8 ? 2048 / kThreads : kThreads == 512 ? 3 : 1;
     static_assert(kN % 8 == 0, "whole groups");
     __device__ static int per_row() { return kL ? kL : int(blockDim.x); }
@@ -190,7 +193,8 @@ __device__ __forceinline__ float read_as(const DenseView& d, int64_t row, int c)
 // Writes the block from column c on again, its scale from the largest |s * root * w| in 64 bits: for a block whose
 // largest value in fp32 is next to a border between scales. One thread, from memory, and a call of its own: a block
 // in a million needs it, and in the kernel's registers it would cost all of them (218 against 191 us for 2^20 rows
-// of 128).
+// of 128). The call takes about 25 us, which shows where it falls to one of the last rows (the same rows: 191 and 215 us;
+// 16384 rows of 4096: 90 and up to 116 us).
 static __device__ __noinline__ void rewrite_block(const RmsNormArgs& a, int64_t row, int c, double root) {
     const float inv = float(root);
     const DenseView weight{const_cast<void*>(a.weight), a.w_dtype, 0};
@@ -304,7 +308,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kForwardBlocks) rms_norm_kerne
 // Persistent blocks over the rows; each thread keeps the weight gradient of its columns in registers
 // and the block writes one row of partial sums to the workspace, in which a second kernel adds the
 // blocks up in their order. Registers are held to 64 a thread: the pass waits for memory, and 1024 threads per SM
-// hide it better than 512 with more registers (rows of 128: 233 against 265 us, of 4096: 234 against 347 us).
+// hide it better than 512 with more registers (rows of 128: 233 against 265 us, of 4096: 234 against 347 us). With sixteen
+// columns a thread that bound spills (see the top); the other side of it is not measured there.
 template <class S, bool kYWide, bool kRWide>
 __global__ void __launch_bounds__(S::kThreads, S::kL ? 4 : 2) rms_norm_grad_kernel(RmsNormGradArgs a) {
     __shared__ float smem[32];
@@ -412,7 +417,8 @@ inline bool aligned16(const DenseView& v) { return aligned(v.p, v.ld * (v.dtype 
 
 // Threads that hold O columns, n each, in whole warps.
 inline int threads_for(int O, int n) { return ((O + n - 1) / n + 31) / 32 * 32; }
-// Threads of a backward block that holds one row (O > 256): 8 columns each up to 4096 columns, 16 up to 8192.
+// Threads of a backward block that holds one row (O > 256): 8 columns each up to 4096 columns, 16 up to 8192 (512
+// threads of 8 hold 4096).
 inline int grad_threads(int O) { return std::min(512, threads_for(O, O <= 4096 ? 8 : 16)); }
 
 template <class S, bool kXWide, bool kRWide>
@@ -439,7 +445,8 @@ cudaError_t forward_spans(const RmsNormArgs& a, cudaStream_t st) {
     if (O <= 256) return launch_norm<Span<kV, 32, 8>, kXWide, kRWide>(a, 0, st);
     if (O <= 512) return launch_norm<Span<kV, 32, 16>, kXWide, kRWide>(a, 0, st);
     if (O <= 1024) return launch_norm<Span<kV, 0, 8, 128>, kXWide, kRWide>(a, threads_for(O, 8), st);
-    // 16 columns a thread: 8 in twice the threads take 107 against 92 us on 16384 rows of 4096, and as long on one row
+    // 16 columns a thread: 8 in twice the threads take 103 against 90 us on 16384 rows of 4096, 68 against 65 us on rows
+    // of 2048, and as long on one row
     if (O <= 8 * 1024) return launch_norm<Span<kV, 0, 16, 512>, kXWide, kRWide>(a, threads_for(O, 16), st);
     if (O <= 16 * 1024) return launch_norm<Span<kV, 0, 16, 1024>, kXWide, kRWide>(a, threads_for(O, 16), st);
     return launch_norm<Span<kV, 0, 0, 1024>, kXWide, kRWide>(a, 1024, st);
