@@ -966,3 +966,28 @@ def test_refusals_are_argument_errors(cuda):
     torch.cuda.synchronize()
     again = vm.add_rms_norm(X, w, residual=X)
     assert torch.equal(again[0].data.view(torch.uint8), Q.data.view(torch.uint8)) and torch.equal(again[1], h) and torch.equal(again[2], inv)
+
+
+def test_mx_tensors_changed_in_place(cuda):
+    """A tensor of an MX matrix that was resized, replaced or turned after the matrix was made is refused by every call, for reading and for
+    writing; values may change."""
+    M, O = 40, 64
+    csr = sparse(M, M, 0.2, 1)
+    dV, w = handle(M, M, *csr, False), torch.ones(O, device="cuda")
+    X, C = torch.randn(M, O, device="cuda"), torch.empty(M, O, device="cuda")
+    changes = (lambda t: t.resize_(4, t.shape[1]), lambda t: t.resize_(M, 1), lambda t: t.resize_(0), lambda t: t.t_(), lambda t: t.unsqueeze_(0),
+               lambda t: t.as_strided_((M, t.shape[1]), (0, 1)), lambda t: t.set_(torch.empty(M // 2, t.shape[1], dtype=t.dtype, device="cuda")))
+    for kind in KINDS.values():
+        for which in ("data", "scale"):
+            for change in changes:
+                Q = vm.mx_quantize(X, kind)
+                change(getattr(Q, which))
+                for call in (lambda: vm.spmm(dV, Q, C), lambda: vm.mx_dequantize(Q), lambda: vm.mx_quantize(X, kind, out=Q),
+                             lambda: vm.add_rms_norm(X, w, kind=kind, out=Q)):
+                    with pytest.raises(vm.VcsrmcError) as e:
+                        call()
+                    assert e.value.status == 1, str(e.value)
+        Q = vm.mx_quantize(X, kind)
+        Q.scale.view(torch.uint8).fill_(127)
+        check_product(dV, csr, *codes_of(Q), "mxf8" if kind == vm.MXF8 else "mxf4", Q=Q)
+    torch.cuda.synchronize()

@@ -150,8 +150,14 @@ Mx mx_new(int64_t rows, int64_t cols, int kind, int device) {
     if (m.lds != blocks) m.scale = m.scale.narrow(1, 0, blocks);
     return m;
 }
-// From five arguments (data, scale, kind, ldq, lds).
-Mx mx_given(PyObject* const* a) {
+// Whether a tensor still holds rows x width elements, its rows ld apart.
+bool holds(const at::Tensor& t, int64_t rows, int64_t width, int64_t ld) {
+    return t.layout() == at::kStrided && t.dim() == 2 && t.element_size() == 1 && t.size(0) == rows && t.size(1) >= width &&
+           (rows <= 1 || t.stride(0) == ld) && (t.size(1) <= 1 || t.stride(1) == 1);
+}
+// From five arguments (data, scale, kind, ldq, lds) that were checked when the matrix was made, and its shape. A tensor may have been
+// changed in place since (resize_, set_, t_), and the kernels would follow the old strides out of it: sizes are looked at again.
+Mx mx_given(PyObject* const* a, int64_t rows, int64_t cols) {
     Mx m;
     m.data = tensor(a[0], "MX elements");
     m.scale = tensor(a[1], "MX scales");
@@ -159,6 +165,9 @@ Mx mx_given(PyObject* const* a) {
     m.ldq = integer(a[3]);
     m.lds = integer(a[4]);
     if (!m.data.is_cuda() || !m.scale.is_cuda()) invalid("microscaled operators run on CUDA tensors");
+    if (!holds(m.data, rows, m.kind == VCSRMC_MXF8 ? cols : (cols + 1) / 2, m.ldq) || !holds(m.scale, rows, (cols + 31) / 32, m.lds) ||
+        m.data.get_device() != m.scale.get_device())
+        invalid("the tensors of an MX matrix were changed after it was made");
     return m;
 }
 PyObject* mx_result(const Mx& m) {
@@ -192,7 +201,7 @@ PyObject* mx_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
         count(n, 7);
         const Matrix x = dense(tensor(a[0], "X"), "X");
         c10::cuda::CUDAGuard guard{c10::DeviceIndex(x.device)};
-        const Mx q = a[2] == Py_None ? mx_new(x.rows, x.cols, int(integer(a[1])), x.device) : mx_given(a + 2);
+        const Mx q = a[2] == Py_None ? mx_new(x.rows, x.cols, int(integer(a[1])), x.device) : mx_given(a + 2, x.rows, x.cols);
         check(vcsrmc_mx_quantize(x.p, x.code, x.ld, x.rows, int32_t(x.cols), q.kind, q.data.data_ptr(), q.ldq, q.s(), q.lds,
                                  stream_of(x.device)));
         return mx_result(q);
@@ -203,8 +212,8 @@ PyObject* mx_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* mx_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&] {
         count(n, 8);
-        const Mx q = mx_given(a);
         const int64_t rows = integer(a[5]), cols = integer(a[6]);
+        const Mx q = mx_given(a, rows, cols);
         const int device = q.data.get_device();
         const Matrix y = dense(tensor(a[7], "out"), "out");
         if (y.rows != rows || y.cols != cols || y.device != device) invalid("out must have Q's shape and device");
@@ -220,8 +229,8 @@ PyObject* spmm_mx(PyObject*, PyObject* const* a, Py_ssize_t n) {
         count(n, 14);
         auto* d = reinterpret_cast<const vcsrmc_device_format*>(integer(a[0]));
         const int device = int(integer(a[1]));
-        const Mx q = mx_given(a + 4);
         const int64_t rows = integer(a[9]), cols = integer(a[10]), O = integer(a[11]);
+        const Mx q = mx_given(a + 4, rows, cols);
         const Matrix c = dense(tensor(a[12], "C"), "C");
         if (c.code != VCSRMC_F32) invalid("C must be float32");
         if (c.device != device || q.data.get_device() != device) invalid("A, B and C must be on the same device");
@@ -259,7 +268,7 @@ PyObject* add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
             o.p = h.data_ptr();
             o.ld = std::max<int64_t>(x.cols, 1);
         }
-        const Mx q = a[5] == Py_None ? mx_new(x.rows, x.cols, int(integer(a[4])), x.device) : mx_given(a + 5);
+        const Mx q = a[5] == Py_None ? mx_new(x.rows, x.cols, int(integer(a[4])), x.device) : mx_given(a + 5, x.rows, x.cols);
         const at::Tensor inv = empty(x.rows, at::kFloat, x.device);
         check(vcsrmc_add_rms_norm(x.p, x.code, x.ld, r.p, r.ld, o.p, o.ld, r.code, w.p, w.code, float(eps), x.rows, int32_t(x.cols), q.kind,
                                   q.data.data_ptr(), q.ldq, q.s(), q.lds, static_cast<float*>(inv.data_ptr()), stream_of(x.device)));
